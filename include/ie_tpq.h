@@ -251,6 +251,75 @@ int ie_rope_kv(const void* qkv, int64_t ld_qkv, int32_t dtype, int64_t tokens, i
                int32_t halved, const int64_t* slots, void* k_cache, void* v_cache,
                int64_t cache_slots, void* q_out, void* stream);
 
+/* ---- attention over the paged cache ----------------------------------------------
+ * No counterpart in the reference's GPU path (its windowed attention is NumPy).
+ * q [tokens][heads][head_dim] attends over the caches [cache_slots][kv_heads]
+ * [head_dim]; key j of sequence s lies in slot
+ * block_tables[s][j / block_size] * block_size + j % block_size.  Query heads
+ * h * heads / kv_heads .. share kv head h.  Sequence s owns the query tokens
+ * [cu_seqlens_q[s], cu_seqlens_q[s + 1]) and its last one is at position
+ * context_lens[s] - 1; with cu_seqlens_q NULL every sequence has one token.
+ *
+ * ie_window_attention: the query at position p sees key j iff j <= p and
+ * (window == 0 or j > p - window or j < sinks).
+ * ie_shared_prefix_attention: j <= p, where the keys below prefix_len are the
+ * same for every sequence and are looked up in the FIRST row of block_tables;
+ * they are read once for the whole batch.
+ *
+ * Both: a query that sees nothing (an empty context) gets zeros.  A key whose
+ * table entry names no page of the cache (-1, as a page given back reads) is not
+ * seen; K and V rows that are not seen may hold anything, NaN included.
+ * Softmax, sums and the join of parts are f32.  f32 rows, head sizes other than
+ * 64 and 128 and rows that are not 16-byte aligned run on the CUDA cores. */
+#define IE_ATTENTION_MAX_HEAD_DIM 256
+typedef struct ie_attention_args {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;    /* elements; a head's elements are adjacent */
+  const void* k_cache;
+  const void* v_cache;
+  int64_t cache_slots, slot_stride, head_stride;  /* strides of both caches, elements */
+  const int32_t* block_tables;
+  int64_t table_stride, table_width;        /* entries */
+  const int32_t* context_lens;              /* [seqs], in device memory */
+  const int32_t* cu_seqlens_q;              /* [seqs + 1], in device memory, or NULL */
+  void* out;                                /* [tokens][heads][head_dim] of q's type */
+  int64_t out_token_stride;
+  int64_t tokens, seqs;
+  int64_t max_query_len, max_context_len;   /* the longest of the batch (0: not known): they
+                                               size the launch, any value gives the result */
+  int64_t window, sinks, prefix_len;
+  void* workspace;                          /* ie_attention_workspace_size bytes, 16-byte
+                                               aligned, no initial contents; calls that
+                                               overlap on the GPU need their own */
+  size_t workspace_bytes;
+  int32_t dtype, heads, kv_heads, head_dim, block_size;
+  float scale;                              /* of the scores, head_dim^-1/2 as a rule */
+} ie_attention_args;
+size_t ie_attention_workspace_size(const ie_attention_args* a);
+int ie_window_attention(const ie_attention_args* a, void* stream);
+int ie_shared_prefix_attention(const ie_attention_args* a, void* stream);
+
+/* ---- pages of the cache ------------------------------------------------------------
+ * Page dst[i] <- page src[i] in each of `ncaches` caches (host array of device
+ * pointers: every layer's K and V) of num_pages pages of page_bytes each.  src
+ * and dst are host arrays and are read before the call returns.  A page that is
+ * out of range, written twice, or both read and written: IE_ERR_INVALID. */
+int ie_copy_pages(void* const* caches, int32_t ncaches, int64_t page_bytes, int64_t num_pages,
+                  const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* ---- log probabilities ----------------------------------------------------------------
+ * For each row of logits [rows][vocab] (row stride ld): the log probability of
+ * tokens[r] (-inf for a token outside the vocabulary), the entropy in nats, and
+ * the `top` largest log probabilities with their tokens, best first, ties to the
+ * lower token (top_* may be NULL when top is 0).  Sums are f32.  A row with a
+ * NaN or +inf logit, or with none above -inf, gives NaN; its top tokens are
+ * still those of its largest logits (NaN ranking with -inf). */
+#define IE_LOGPROBS_MAX_TOP 64
+#define IE_LOGPROBS_MAX_VOCAB 2097152
+int ie_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int64_t rows, int64_t vocab,
+                      const int64_t* tokens, int32_t top, float* logprobs, float* entropy,
+                      float* top_logprobs, int64_t* top_tokens, void* stream);
+
 /* ---- all_reduce over a list of partials in one process -----------------------
  * Replaces ie/parallel/sharding.py:40-44: out = p[0] + p[1] + ... in rank order
  * (f32 arithmetic, the reference's order).  dtype applies to inputs and out. */

@@ -1,0 +1,120 @@
+// Shared pieces of the paged attention kernels: the launch parameters, which
+// keys a query sees, and where a key's row lies in the cache.
+#pragma once
+
+#include "common.cuh"
+
+namespace ie {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// n / d for 0 <= n < 2^31 by a multiplication and a shift, d fixed on the host
+// (Granlund and Montgomery, Division by Invariant Integers using Multiplication).
+struct FastDiv {
+  uint32_t mul = 1, shift = 0, d = 1;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div) {
+    while ((1ull << shift) < div) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - div)) / div + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((__umulhi(mul, (uint32_t)n) + (uint32_t)n) >> shift);
+  }
+};
+
+struct Params {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_token, q_head;        // strides in elements
+  int64_t out_token;
+  int64_t slot_stride, head_stride;   // of both caches
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* context;
+  const int32_t* cu_q;            // null: one token per sequence
+  int tokens, seqs, heads, kv_heads, group, hd;
+  int table_width, pages;
+  FastDiv block, group_div;
+  int window, sinks;              // window 0: every earlier key
+  int prefix;                     // keys below it are looked up in the first table row
+  int key_start, key_end;         // only keys in [key_start, key_end) (a part of the softmax)
+  float scale2;                   // softmax scale * log2 e
+  // Parts of a row's softmax: [token * heads + head][slots] partial results, of
+  // which this launch writes [slot0, slot0 + parts).  part_o holds the sum
+  // relative to 2^m, part_ml (m, l); l = 0 means nothing was seen and part_o
+  // is not written.  slots = 0: the launch covers every key and writes `out`.
+  float* part_o;
+  float2* part_ml;
+  int slots, slot0, parts;
+};
+
+// Cache row of `key`, or -1 when the table names no page of the cache there.
+__device__ __forceinline__ int cache_slot(const Params& p, const int32_t* table, int key) {
+  const int page_no = p.block.div(key);
+  if (page_no >= p.table_width) return -1;
+  const int page = __ldg(table + page_no);
+  if (page < 0 || page >= p.pages) return -1;
+  return page * (int)p.block.d + (key - page_no * (int)p.block.d);
+}
+
+// Sequence of query token t: the last s with cu_q[s] <= t.
+__device__ __forceinline__ int sequence_of(const Params& p, int t) {
+  if (!p.cu_q) return t;
+  int lo = 0, hi = p.seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(p.cu_q + mid) <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Context length of sequence s, held to what its table row can address.
+__device__ __forceinline__ int context_of(const Params& p, int s) {
+  const int64_t most = (int64_t)p.table_width * p.block.d;
+  const int c = __ldg(p.context + s);
+  return c < 0 ? 0 : (c < most ? c : (int)most);
+}
+
+// Position of query token t of sequence s; negative: it sees nothing.
+__device__ __forceinline__ int position_of(const Params& p, int s, int t) {
+  const int ctx = context_of(p, s);
+  if (!p.cu_q) return ctx - 1;
+  return ctx - (__ldg(p.cu_q + s + 1) - t);
+}
+
+// The keys that a query at `pos` sees within [key_start, key_end), numbered
+// 0 .. n-1: the sinks in front of the window first, then [lo, lo + n - ns).
+struct Keys {
+  int ns, lo, n;
+  __device__ __forceinline__ int at(int i) const { return i < ns ? i : lo + (i - ns); }
+};
+__device__ __forceinline__ Keys keys_of(const Params& p, int pos) {
+  Keys k;
+  int lo = p.key_start;
+  if (p.window > 0 && pos - p.window + 1 > lo) lo = pos - p.window + 1;
+  k.lo = lo;
+  k.ns = p.key_start == 0 ? min(p.sinks, lo) : 0;
+  const int hi = min(pos + 1, p.key_end);
+  k.n = k.ns + max(hi - lo, 0);
+  if (pos < 0) k.n = k.ns = 0;
+  return k;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- launchers -------------------------------------------------------------
+// Any type, head size up to 256 and alignment (attention_simt.cu).
+int launch_simt(const Params& p, int dtype, cudaStream_t s);
+// out = the joined parts [0, slots) of every row.
+int launch_join(const Params& p, int dtype, cudaStream_t s);
+
+}  // namespace attn
+}  // namespace ie

@@ -45,6 +45,9 @@ IE_AR_AUTO, IE_AR_ONESHOT, IE_AR_TWOSHOT, IE_AR_NVLS = 0, 1, 2, 3
 
 IE_COMM_HANDLE_BYTES = 64
 IE_QLINEAR_NOALLOC_SCRATCH_BYTES = 8 << 20
+IE_ATTENTION_MAX_HEAD_DIM = 256
+IE_LOGPROBS_MAX_TOP = 64
+IE_LOGPROBS_MAX_VOCAB = 2097152
 
 # every symbol include/ie_tpq.h declares
 EXPORTED = (
@@ -52,6 +55,8 @@ EXPORTED = (
     "ie_round_to_float_format", "ie_pack_weight", "ie_dequantize",
     "ie_qlinear_workspace_size", "ie_qlinear", "ie_qlinear_noalloc", "ie_kernel_status",
     "ie_rms_norm", "ie_rope_kv",
+    "ie_attention_workspace_size", "ie_window_attention", "ie_shared_prefix_attention",
+    "ie_copy_pages", "ie_token_logprobs",
     "ie_reduce_partials", "ie_comm_create",
     "ie_comm_export", "ie_comm_open", "ie_comm_destroy", "ie_comm_set_timeout",
     "ie_comm_check", "ie_qlinear_allreduce", "ie_allreduce", "ie_allreduce_resolve",
@@ -95,6 +100,41 @@ class QLinearArgs(ctypes.Structure):
     ]
 
 
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("cache_slots", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("block_tables", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("context_lens", ctypes.c_void_p),
+        ("cu_seqlens_q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_token_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("seqs", ctypes.c_int64),
+        ("max_query_len", ctypes.c_int64),
+        ("max_context_len", ctypes.c_int64),
+        ("window", ctypes.c_int64),
+        ("sinks", ctypes.c_int64),
+        ("prefix_len", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _lib: ctypes.CDLL | None = None
 _load_error: str | None = None
 
@@ -121,6 +161,13 @@ def _declare(lib: ctypes.CDLL) -> None:
                                        ctypes.c_float, _P]),
         "ie_rope_kv": (ctypes.c_int, [_P, _I64, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _I64,
                                       _I32, _P, _P, _P, _I64, _P, _P]),
+        "ie_attention_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
+        "ie_window_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _P]),
+        "ie_shared_prefix_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _P]),
+        "ie_copy_pages": (ctypes.c_int, [ctypes.POINTER(_P), _I32, _I64, _I64, _P, _P, _I64,
+                                         _P]),
+        "ie_token_logprobs": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _P, _I32, _P, _P, _P,
+                                             _P, _P]),
         "ie_reduce_partials": (ctypes.c_int, [ctypes.POINTER(_P), _I32, _P, _I64, _I32, _P]),
         "ie_comm_create": (ctypes.c_int, [_I32, _I32, _I32, ctypes.c_size_t,
                                           ctypes.POINTER(_P)]),

@@ -1,0 +1,52 @@
+"""Log probabilities of given tokens, with the entropy and the best alternatives
+of every row (``ie_token_logprobs``)."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+from . import _lib
+from .device import dtype_code, require_cuda
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: "torch.Tensor"        # f32 [rows]
+    entropy: "torch.Tensor"         # f32 [rows], nats
+    top_logprobs: "torch.Tensor"    # f32 [rows, top], best first
+    top_tokens: "torch.Tensor"      # int64 [rows, top], ties to the lower token
+
+
+def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
+    """``log softmax(logits)[r, tokens[r]]``, the rows' entropies and their ``top``
+    (at most 64) largest log probabilities, in one pass over the logits.
+
+    logits: CUDA ``[rows, vocab]`` (f32 / bf16 / f16), rows of any stride.  tokens:
+    int64 ``[rows]``; one outside the vocabulary has log probability -inf.
+    Logits of -inf (a vocabulary mask) are allowed; a row with a NaN or +inf, or
+    with no logit above -inf, gives NaN.
+    """
+    torch = require_cuda()
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be a row-contiguous 2-D tensor")
+    rows, vocab = logits.shape
+    if tokens.dtype != torch.long or tokens.dim() != 1 or tokens.shape[0] != rows or \
+            not tokens.is_contiguous():
+        raise ValueError("tokens must be a contiguous int64 tensor of one entry per row")
+    if logits.get_device() < 0 or tokens.get_device() != logits.get_device():
+        raise ValueError("logits and tokens must be on one CUDA device")
+    if not 0 <= top <= min(vocab, _lib.IE_LOGPROBS_MAX_TOP):
+        raise ValueError(f"top={top} outside [0, min({_lib.IE_LOGPROBS_MAX_TOP}, {vocab})]")
+    if logits.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(logits.get_device()):
+            return token_logprobs(logits, tokens, top, stream)
+    if stream is not None and stream != torch.cuda.current_stream():
+        with torch.cuda.stream(stream):   # the outputs belong to that stream
+            return token_logprobs(logits, tokens, top)
+    device = logits.device
+    both = torch.empty((2, rows), dtype=torch.float32, device=device)
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+    top_tokens = torch.empty((rows, top), dtype=torch.long, device=device)
+    _lib.check(_lib.lib().ie_token_logprobs(
+        logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), rows, vocab,
+        tokens.data_ptr(), top, both.data_ptr(), both.data_ptr() + 4 * rows,
+        top_logprobs.data_ptr(), top_tokens.data_ptr(), _lib.stream_ptr()), "token_logprobs")
+    return TokenLogprobs(both[0], both[1], top_logprobs, top_tokens)

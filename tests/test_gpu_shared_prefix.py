@@ -1,0 +1,125 @@
+"""``shared_prefix_attention`` against the f64 definition: decode and several
+queries a sequence, prefixes around page and tile edges, sequences shorter than
+the prefix, NaN where nothing may be read, and refusals."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from ie_tpq.kv_attention import shared_prefix_attention, window_attention
+from tests.attention_oracle import Batch, assert_close
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def check(b, **kw):
+    got = shared_prefix_attention(b.q, b.k, b.v, b.tables, b.ctx, b.prefix, b.block,
+                                  **{**b.lens(), **kw})
+    want, weight, largest = b.oracle(prefix=b.prefix)
+    assert_close(got, want, weight, largest, b.q.shape[2])
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (64, 8, 128), (14, 2, 64), (4, 4, 128),
+                                         (4, 2, 8), (5, 1, 80)])
+def test_decode(dtype, heads, kv, hd):
+    check(Batch([200, 161, 250, 330], heads, kv, hd, dtype, 16, prefix=160, seed=hd))
+
+
+@pytest.mark.parametrize("prefix", [0, 1, 15, 16, 17, 127, 128, 129, 300, 1000, 2048])
+def test_prefix_lengths(prefix):
+    """Prefixes that end inside a page: the shared part is read through the first
+    row, the rest of that page through each sequence's own."""
+    check(Batch([prefix + n for n in (1, 9, 140)], 8, 2, 128, BF16, 16, prefix=prefix,
+                seed=prefix))
+
+
+@pytest.mark.parametrize("seqs", [1, 2, 31, 33, 70])
+def test_batch_sizes(seqs):
+    check(Batch([140 + i for i in range(seqs)], 8, 2, 64, F16, 16, prefix=130, seed=seqs))
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16), (64, F32)])
+def test_several_queries(hd, dtype):
+    query = [1, 7, 40, 0, 3]
+    check(Batch([100 + n for n in query], 8, 2, hd, dtype, 16, query=query, prefix=96, seed=hd))
+
+
+def test_sequences_shorter_than_the_prefix():
+    b = Batch([100, 20, 1, 0, 64], 8, 2, 64, BF16, 16, prefix=64, seed=3)
+    got = check(b)
+    assert torch.count_nonzero(got[3]) == 0
+    check(Batch([100, 20, 60], 8, 2, 128, BF16, 16, query=[10, 20, 30], prefix=64, seed=4))
+
+
+def test_the_first_row_names_the_prefix():
+    b = Batch([90, 95, 70], 8, 2, 128, BF16, 16, prefix=64, seed=5)
+    want = check(b)
+    b.tables[1:, :4] = -1        # not read
+    assert torch.equal(check(b), want)
+
+
+def test_equal_to_attention_over_whole_tables():
+    b = Batch([700, 650, 640], 8, 2, 128, BF16, 16, prefix=640, seed=6)
+    check(b)
+    got = window_attention(b.q, b.k, b.v, b.tables, b.ctx, 16, **b.lens())
+    want, weight, largest = b.oracle(prefix=640)
+    assert_close(got, want, weight, largest, 128)
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16), (64, F32)])
+def test_values_that_a_sequence_does_not_see(hd, dtype):
+    """A value that is NaN poisons the sequences whose context reaches it alone."""
+    b = Batch([60, 30, 64], 8, 2, hd, dtype, 16, prefix=48, seed=7)
+    want, weight, largest = b.oracle(prefix=48)
+    slot = int(b.tables[0, 2]) * 16 + 8                    # position 40
+    b.v[slot] = float("nan")
+    got = shared_prefix_attention(b.q, b.k, b.v, b.tables, b.ctx, 48, 16, **b.lens())
+    assert_close(got[1:2], want[1:2], weight[1:2], largest, hd)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[2]).all()
+
+
+@pytest.mark.parametrize("lens", [dict(max_query_len=0, max_context_len=0),
+                                  dict(max_query_len=1, max_context_len=1),
+                                  dict(max_query_len=999, max_context_len=99999)])
+@pytest.mark.parametrize("query", [None, [3, 40]])
+def test_lengths_unknown_or_wrong_give_the_same(lens, query):
+    check(Batch([500, 800], 8, 2, 128, F16, 16, query=query, prefix=400, seed=8), **lens)
+
+
+def test_large_scores_and_same_bits():
+    b = Batch([1500, 1600, 1501], 32, 8, 128, F16, 16, prefix=1400, seed=9, std=20.0)
+    assert torch.equal(check(b), check(b))
+
+
+def test_graph_capture():
+    b = Batch([300, 290], 8, 2, 128, BF16, 16, prefix=256, seed=10)
+    call = lambda: shared_prefix_attention(b.q, b.k, b.v, b.tables, b.ctx, 256, 16, **b.lens())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    b.q.copy_(b.q.flip(0))
+    graph.replay()
+    want, weight, largest = b.oracle(prefix=256)
+    assert_close(out, want, weight, largest, 128)
+
+
+def test_refusals():
+    b = Batch([50, 60], 4, 2, 64, BF16, 16, prefix=32, seed=11)
+    args = (b.q, b.k, b.v, b.tables, b.ctx)
+    for prefix in (-1, 65, 2 ** 40):
+        with pytest.raises(ValueError):
+            shared_prefix_attention(*args, prefix, 16)
+    with pytest.raises(ValueError):
+        shared_prefix_attention(*args, 32, 0)
+    with pytest.raises(ValueError):
+        shared_prefix_attention(b.q[:1], *args[1:], 32, 16)
+    assert np.isfinite(b.q.float().cpu().numpy()).all()

@@ -1,0 +1,269 @@
+"""``window_attention`` against the f64 definition (tests/attention_oracle.py):
+decode and ragged prefill, every type, head layouts and sizes, windows and
+sinks around their edges, pages that end inside a tile, rows that see nothing,
+NaN where nothing may be read, strides, streams and refusals."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from ie_tpq.kv_attention import window_attention
+from tests.attention_oracle import Batch, as_f64, assert_close, attention
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def check(b, window=0, sinks=0, **kw):
+    got = window_attention(b.q, b.k, b.v, b.tables, b.ctx, b.block, window=window, sinks=sinks,
+                           **b.lens(), **kw)
+    want, weight, largest = b.oracle(window=window, sinks=sinks)
+    assert_close(got, want, weight, largest, b.q.shape[2])
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (14, 2, 64), (8, 8, 128), (4, 2, 8),
+                                         (20, 1, 64), (5, 1, 80), (3, 3, 256)])
+def test_decode(dtype, heads, kv, hd):
+    b = Batch([300, 1, 0, 77, 128, 129], heads, kv, hd, dtype, 16, seed=hd)
+    check(b)
+    check(b, window=50, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (14, 2, 64), (2, 2, 128), (4, 2, 8),
+                                         (20, 1, 64), (5, 1, 80)])
+def test_prefill(dtype, heads, kv, hd):
+    b = Batch([70, 1, 0, 133, 40], heads, kv, hd, dtype, 16, query=[70, 1, 0, 5, 33], seed=hd)
+    check(b)
+    check(b, window=31, sinks=2)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 200), (16, 0), (100, 4), (128, 128),
+                                          (129, 17), (200, 1), (201, 5), (100000, 7),
+                                          (1 << 40, 1 << 40)])
+@pytest.mark.parametrize("query", [None, [1, 200, 30]])
+def test_window_edges(window, sinks, query):
+    b = Batch([64, 200, 199], 8, 2, 128, BF16, 16, query=query, seed=window % 97)
+    check(b, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("block", [1, 5, 16, 48, 128, 256])
+@pytest.mark.parametrize("query", [None, [100, 3, 260]])
+def test_pages(block, query):
+    b = Batch([100, 1000, 300], 4, 2, 64, F16, block, query=query, seed=block)
+    check(b)
+    check(b, window=90, sinks=4)
+
+
+@pytest.mark.parametrize("context", [1, 127, 128, 129, 511, 2049])
+def test_decode_splits(context):
+    """One sequence: its keys are split over the SMs and joined."""
+    b = Batch([context], 8, 2, 128, BF16, 16, seed=context)
+    check(b)
+    check(b, window=max(1, context // 2), sinks=4)
+
+
+def test_chunked_prefill_equals_whole_prefill_rows():
+    """The last queries of a prompt attend alike as a chunk and within the whole."""
+    whole = Batch([300], 8, 2, 128, BF16, 16, query=[300], seed=5)
+    got = check(whole, window=100, sinks=4)
+    part = window_attention(whole.q[260:], whole.k, whole.v, whole.tables, whole.ctx, 16,
+                            window=100, sinks=4, max_query_len=40, max_context_len=300,
+                            cu_seqlens_q=torch.tensor([0, 40], dtype=torch.int32, device="cuda"))
+    want, weight, largest = whole.oracle(window=100, sinks=4)
+    assert_close(part, want[260:], weight[260:], largest, 128)
+    assert got.shape == whole.q.shape
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (F16, 64), (F32, 64)])
+@pytest.mark.parametrize("query", [None, [2, 4]])
+def test_lengths_unknown_or_wrong_give_the_same(dtype, hd, query):
+    b = Batch([500, 300], 8, 2, hd, dtype, 16, query=query, seed=2)
+    want, weight, largest = b.oracle()
+    for lens in (dict(), dict(max_query_len=1, max_context_len=1),
+                 dict(max_query_len=10000, max_context_len=100000)):
+        got = window_attention(b.q, b.k, b.v, b.tables, b.ctx, 16, cu_seqlens_q=b.cu, **lens)
+        assert_close(got, want, weight, largest, hd)
+
+
+@pytest.mark.parametrize("query", [None, [7, 9]])
+def test_query_longer_than_its_context_sees_nothing_before_it(query):
+    b = Batch([40, 3], 8, 2, 64, BF16, 16, query=query, seed=3)
+    got = check(b)
+    if query:
+        assert torch.count_nonzero(got[7:13]) == 0 and torch.count_nonzero(got[13:]) > 0
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16), (64, F32)])
+@pytest.mark.parametrize("query", [None, [60]])
+def test_entries_outside_the_cache_hide_their_keys(hd, dtype, query):
+    b = Batch([200], 8, 2, hd, dtype, 16, query=query, seed=4)
+    b.tables[0, 3] = -1
+    b.tables[0, 5] = b.k.shape[0] // 16
+    b.tables[0, 9] = 2 ** 31 - 1
+    check(b)
+    b.tables[0, :] = -1
+    assert torch.count_nonzero(check(b)) == 0
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16), (64, F32)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_values_behind_the_mask_do_not_matter(hd, dtype, bad):
+    """A broken key or value poisons only the queries that see it."""
+    b = Batch([180], 8, 2, hd, dtype, 16, query=[180], seed=6)
+    want, weight, largest = b.oracle(window=40, sinks=2)
+    at = 100
+    slot = int(b.tables[0, at // 16]) * 16 + at % 16
+    b.v[slot] = bad
+    b.k[slot, 0] = float("nan")
+    got = window_attention(b.q, b.k, b.v, b.tables, b.ctx, 16, window=40, sinks=2, **b.lens())
+    blind = np.r_[0:at, at + 40:180]
+    assert_close(got[blind], want[blind], weight[blind], largest, hd)
+    assert not torch.isfinite(got[at:at + 40]).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_large_scores(dtype):
+    """Scores of several hundred: the maximum is subtracted before the exponential,
+    and a maximum that grows late rescales what was summed before."""
+    for query in (None, [150, 170]):
+        b = Batch([150, 400], 8, 2, 128, dtype, 16, query=query, seed=8, std=20.0)
+        check(b)
+    b = Batch([700], 4, 1, 64, dtype, 16, query=[700], seed=9)
+    ramp = torch.linspace(0, 6, 700, device="cuda")
+    order = (b.tables[0].long()[torch.arange(700, device="cuda") // 16] * 16
+             + torch.arange(700, device="cuda") % 16)
+    b.k[order] = (b.k[order].float() + ramp[:, None, None] * b.q[-1, 0].float()).to(dtype)
+    check(b)
+
+
+def test_strides():
+    """q as a slice of the fused projection, caches as halves of one tensor, a table
+    that is a slice, and an output with wider rows."""
+    b = Batch([90, 33], 8, 2, 64, BF16, 16, query=[20, 33], seed=10)
+    want, weight, largest = b.oracle(window=30, sinks=1)
+    wide = torch.zeros((53, 12, 64), dtype=BF16, device="cuda")
+    wide[:, 2:10] = b.q
+    both = torch.stack([b.k, b.v], dim=1)
+    tables = torch.full((2, 40), -1, dtype=torch.int32, device="cuda")
+    tables[:, 3:3 + b.tables.shape[1]] = b.tables
+    out = torch.zeros((53, 10, 64), dtype=BF16, device="cuda")[:, 1:9]
+    got = window_attention(wide[:, 2:10], both[:, 0], both[:, 1],
+                           tables[:, 3:3 + b.tables.shape[1]], b.ctx, 16, window=30, sinks=1,
+                           out=out, **b.lens())
+    assert got is out
+    assert_close(got, want, weight, largest, 64)
+
+
+@pytest.mark.parametrize("query", [None, [20, 33]])
+def test_rows_that_are_not_aligned(query):
+    b = Batch([90, 33], 4, 2, 64, F16, 16, query=query, seed=11)
+    want, weight, largest = b.oracle()
+    flat = torch.zeros(b.q.numel() + 1, dtype=F16, device="cuda")
+    q = flat[1:].view(b.q.shape)
+    q.copy_(b.q)
+    got = window_attention(q, b.k, b.v, b.tables, b.ctx, 16, **b.lens())
+    assert_close(got, want, weight, largest, 64)
+
+
+def test_scale():
+    b = Batch([90, 33], 4, 2, 64, BF16, 16, seed=12)
+    got = window_attention(b.q, b.k, b.v, b.tables, b.ctx, 16, scale=0.3)
+    want, weight, largest = b.oracle(scale=0.3)
+    assert_close(got, want, weight, largest, 64)
+
+
+def test_cache_beyond_32_bit_offsets():
+    """A page behind the first 2^31 elements (and 2^32 bytes) of the cache."""
+    block, kv, hd = 256, 8, 128
+    slots = (2 ** 31 // (kv * hd) // block + 4) * block
+    k = torch.zeros((slots, kv, hd), dtype=BF16, device="cuda")
+    v = torch.zeros_like(k)
+    pages = slots // block
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(0)
+    table = torch.tensor([[pages - 1, 0, pages - 3]], dtype=torch.int32, device="cuda")
+    for page in (pages - 1, 0, pages - 3):
+        for c in (k, v):
+            c[page * block:(page + 1) * block].normal_(generator=gen)
+    for n in (1, 50):
+        q = torch.randn((n, 32, hd), generator=gen, device="cuda").to(BF16)
+        ctx = torch.tensor([700], dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        got = window_attention(q, k, v, table, ctx, block, window=500, sinks=4, cu_seqlens_q=cu,
+                               max_query_len=n)
+        near = torch.cat([k[(pages - 1) * block:], k[:block], k[(pages - 3) * block:][:block]])
+        nearv = torch.cat([v[(pages - 1) * block:], v[:block], v[(pages - 3) * block:][:block]])
+        want, weight, largest = attention(q, near, nearv, torch.tensor([[0, 1, 2]]), [700], block,
+                                          query=[n], window=500, sinks=4)
+        assert_close(got, want, weight, largest, hd)
+
+
+def test_same_bits_twice_and_on_another_stream():
+    b = Batch([700, 3000], 8, 2, 128, BF16, 16, seed=13)
+    a = check(b, window=1000, sinks=4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    c = window_attention(b.q, b.k, b.v, b.tables, b.ctx, 16, window=1000, sinks=4, stream=side,
+                         **b.lens())
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("query", [None, [20, 90]])
+def test_graph_capture_follows_the_lengths(query):
+    b = Batch([300, 90], 8, 2, 128, BF16, 16, query=query, seed=14)
+    lens = b.lens()
+    call = lambda: window_attention(b.q, b.k, b.v, b.tables, b.ctx, 16, window=64, sinks=4, **lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    b.context = [211, 90]
+    b.ctx.copy_(torch.tensor(b.context, dtype=torch.int32))
+    graph.replay()
+    want, weight, largest = b.oracle(window=64, sinks=4)
+    assert_close(out, want, weight, largest, 128)
+
+
+def test_empty_batches():
+    b = Batch([5], 4, 2, 64, BF16, 16, seed=15)
+    none = torch.empty((0,), dtype=torch.int32, device="cuda")
+    out = window_attention(b.q[:0], b.k, b.v, b.tables[:0], none, 16)
+    assert out.shape == (0, 4, 64)
+    got = window_attention(b.q, b.k, b.v, b.tables[:, :0], b.ctx, 16)
+    assert torch.count_nonzero(got) == 0
+    got = window_attention(b.q, b.k[:0], b.v[:0], b.tables, b.ctx, 16)
+    assert torch.count_nonzero(got) == 0
+
+
+def test_refusals():
+    b = Batch([50, 20], 4, 2, 64, BF16, 16, seed=16)
+    ok = (b.q, b.k, b.v, b.tables, b.ctx, 16)
+    window_attention(*ok)
+    bad = [
+        (b.q[0], *ok[1:]), (b.q.half(), *ok[1:]), (b.q[:, :3], *ok[1:]), (b.q[..., :32], *ok[1:]),
+        (b.q, b.k[:, :1], *ok[2:]), (b.q, b.k, b.v.half(), *ok[3:]),
+        (*ok[:3], b.tables.long(), *ok[4:]), (*ok[:3], b.tables[0], *ok[4:]),
+        (*ok[:4], b.ctx.long(), 16), (*ok[:4], b.ctx[:1], 16), (*ok[:5], 0),
+        (b.q[:1], *ok[1:]), (b.q.cpu(), *ok[1:]), (*ok[:4], b.ctx.cpu(), 16),
+        (*ok[:5], 2 ** 30),
+    ]
+    for args in bad:
+        with pytest.raises(ValueError):
+            window_attention(*args)
+    for kw in (dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(max_query_len=-1),
+               dict(cu_seqlens_q=b.ctx), dict(out=b.q[:1]), dict(window=1.5)):
+        with pytest.raises(ValueError):
+            window_attention(*ok, **kw)
+    big = torch.zeros((1, 2, 512), dtype=BF16, device="cuda")
+    with pytest.raises(ValueError):
+        window_attention(big, big.expand(16, 2, 512).contiguous(),
+                         big.expand(16, 2, 512).contiguous(), b.tables[:1], b.ctx[:1], 16)
