@@ -8,8 +8,6 @@ namespace ie {
 namespace attn {
 namespace {
 
-constexpr int kSms = 148;
-
 int validate(const ie_attention_args& a, const char* who) {
   IE_CHECK(a.dtype == IE_DT_BF16 || a.dtype == IE_DT_F16 || a.dtype == IE_DT_F32,
            "%s: unsupported dtype %d", who, a.dtype);
@@ -17,10 +15,12 @@ int validate(const ie_attention_args& a, const char* who) {
            "%s: %d query heads over %d kv heads", who, a.heads, a.kv_heads);
   IE_CHECK(a.head_dim > 0 && a.head_dim <= IE_ATTENTION_MAX_HEAD_DIM,
            "%s: a head size of %d outside [1, %d]", who, a.head_dim, IE_ATTENTION_MAX_HEAD_DIM);
-  IE_CHECK(a.tokens >= 0 && a.tokens < (1ll << 31) / 256, "%s: %lld query tokens", who,
+  // the launches number (token, head, part) and (row tile, head, part) in 31 bits
+  IE_CHECK(a.tokens >= 0 && a.tokens * a.heads < (1ll << 31) / 128, "%s: %lld query tokens", who,
            (long long)a.tokens);
-  IE_CHECK(a.seqs >= 0 && a.seqs <= a.tokens + (1 << 20), "%s: %lld sequences", who,
-           (long long)a.seqs);
+  IE_CHECK(a.seqs >= 0 && a.seqs <= a.tokens + (1 << 20) &&
+               a.seqs * (int64_t)a.heads < (1ll << 31) / 256,
+           "%s: %lld sequences", who, (long long)a.seqs);
   IE_CHECK(a.cu_seqlens_q || a.seqs == a.tokens,
            "%s: %lld tokens of %lld sequences need cu_seqlens_q", who, (long long)a.tokens,
            (long long)a.seqs);
@@ -33,7 +33,7 @@ int validate(const ie_attention_args& a, const char* who) {
   IE_CHECK(a.max_query_len >= 0 && a.max_context_len >= 0, "%s: negative lengths", who);
   IE_CHECK(a.window >= 0 && a.sinks >= 0 && a.prefix_len >= 0,
            "%s: negative window, sinks or prefix", who);
-  IE_CHECK(a.scale == a.scale && a.scale - a.scale == 0.0f, "%s: the scale is not finite", who);
+  IE_CHECK(a.scale > 0.0f && a.scale - a.scale == 0.0f, "%s: the scale is not positive", who);
   if (a.tokens == 0) return IE_OK;
   IE_CHECK(a.q && a.out && (a.block_tables || a.table_width == 0) && a.context_lens, "%s: null pointer", who);
   IE_CHECK(a.cache_slots == 0 || (a.k_cache && a.v_cache), "%s: null cache", who);
@@ -81,26 +81,91 @@ Params base_params(const ie_attention_args& a) {
   return p;
 }
 
-// Keys that the longest row sees.
-int64_t longest(const ie_attention_args& a) {
-  int64_t n = a.table_width * a.block_size;
-  if (a.max_context_len > 0) n = std::min(n, a.max_context_len);
-  if (a.window > 0) n = std::min(n, a.window + a.sinks);
-  return n;
+bool aligned16(const void* at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; }
+
+// 16-bit rows that the tensor-core kernels read and write as 16-byte vectors.
+bool tensor_cores(const ie_attention_args& a) {
+  const int64_t strides = a.q_token_stride | a.q_head_stride | a.slot_stride | a.head_stride |
+                          a.out_token_stride;
+  return a.dtype != IE_DT_F32 && (a.head_dim == 64 || a.head_dim == 128) && strides % 8 == 0 &&
+         aligned16(a.q) && aligned16(a.k_cache) && aligned16(a.v_cache) && aligned16(a.out) &&
+         a.tokens * (a.heads / a.kv_heads) < (1ll << 31) - 512;
 }
 
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How one call runs: the kernels' parts of a row, and the slots they fill.
 struct Plan {
-  int simt_parts;      // parts of the SIMT kernel
-  int slots;           // 0: written to out directly
+  bool simt, decode, prefix;        // which kernels
+  int simt_parts;
+  int decode_parts, decode_per;     // one token per sequence, own keys
+  bool twin, prefix_twin;           // row tiles: own keys, shared prefix
+  int row_tiles, tile_parts, prefix_row_tiles, prefix_parts;
+  int slots;                        // 0: a single part, written to out directly
 };
+
+// Parts of rows that see up to n keys, for `units` independent rows' worth of work
+// and `wide` CTAs at once: the fewest rounds of CTAs, where a CTA costs its
+// keys and `fixed` more (its start and end), and joining parts costs `join`.
+int best_parts(int64_t units, int64_t n, int64_t step, int wide, int64_t fixed, int64_t join) {
+  int64_t best = 1, least = -1;
+  const int64_t most = std::min<int64_t>(std::max<int64_t>(1, n / step), 128);
+  for (int64_t parts = 1; parts <= most; ++parts) {
+    const int64_t per = ceil_div(ceil_div(n, step), parts) * step;
+    const int64_t cost = ceil_div(units * parts, wide) * (per + fixed) +
+                         (parts > 1 ? join + 4 * parts : 0);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = parts;
+    }
+  }
+  return (int)best;
+}
 
 Plan make_plan(const ie_attention_args& a) {
   Plan plan{};
-  // enough CTAs for every SM's warps, at least 64 keys each
-  const int64_t rows = a.tokens * a.heads;
-  const int64_t want = (kSms * 16 + rows - 1) / rows;
-  plan.simt_parts = (int)std::max<int64_t>(1, std::min(want, longest(a) / 64));
-  plan.slots = plan.simt_parts > 1 ? plan.simt_parts : 0;
+  const int64_t group = a.heads / a.kv_heads;
+  int64_t keys = a.table_width * a.block_size;      // of the longest context
+  if (a.max_context_len > 0) keys = std::min(keys, a.max_context_len);
+  const int64_t seen = a.window > 0 ? std::min(keys, a.window + a.sinks) : keys;
+  if (!tensor_cores(a)) {
+    // enough CTAs for every SM's warps, at least 64 keys each
+    plan.simt = true;
+    const int64_t rows = a.tokens * a.heads;
+    plan.simt_parts = (int)std::max<int64_t>(
+        1, std::min({ceil_div(kSms * 16, rows), seen / 64, (int64_t)1024}));
+    plan.slots = plan.simt_parts > 1 ? plan.simt_parts : 0;
+    return plan;
+  }
+  plan.prefix = a.prefix_len > 0;
+  if (plan.prefix) {
+    const int64_t rows = a.tokens * group;
+    plan.prefix_twin = rows <= 128;
+    plan.prefix_row_tiles = (int)ceil_div(rows, plan.prefix_twin ? 128 : 256);
+    plan.prefix_parts = best_parts(plan.prefix_row_tiles * a.kv_heads, a.prefix_len, 128, kSms,
+                                   256, 512);
+  }
+  const int64_t own = std::max<int64_t>(1, seen - a.prefix_len);
+  if (!a.cu_seqlens_q) {
+    plan.decode = true;
+    const int64_t units = a.seqs * a.kv_heads * ceil_div(group, 16);
+    // 64 keys of a CTA cost about what its start does, a join about 100
+    plan.decode_parts = best_parts(units, own, 64, 2 * kSms, 64, plan.prefix ? 0 : 100);
+    plan.decode_per = (int)(ceil_div(ceil_div(own, 64), plan.decode_parts) * 64);
+    plan.slots = plan.decode_parts;
+  } else {
+    const int64_t queries = a.max_query_len > 0 ? std::min(a.max_query_len, a.tokens) : a.tokens;
+    const int64_t rows = queries * group;
+    plan.twin = rows <= 128 && own > 128;
+    plan.row_tiles = (int)ceil_div(rows, plan.twin ? 128 : 256);
+    // a row tile sees the window of its first token and what lies up to its last
+    const int64_t n = a.window > 0 ? std::min(own, seen + ceil_div(256, group)) : own;
+    plan.tile_parts = best_parts(plan.row_tiles * a.seqs * a.kv_heads, n, 128, kSms, 256,
+                                 plan.prefix ? 0 : 512);
+    plan.slots = plan.tile_parts * (plan.twin ? 2 : 1);
+  }
+  if (plan.prefix) plan.slots += plan.prefix_parts * (plan.prefix_twin ? 2 : 1);
+  if (plan.slots == 1) plan.slots = 0;
   return plan;
 }
 
@@ -113,17 +178,35 @@ int run(const ie_attention_args& a, const char* who, cudaStream_t s) {
   const size_t need = part_bytes(a, plan.slots);
   IE_CHECK(need == 0 || (a.workspace && a.workspace_bytes >= need),
            "%s: a workspace of %zu bytes < %zu", who, a.workspace_bytes, need);
-  IE_CHECK(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "%s: unaligned workspace", who);
+  IE_CHECK(aligned16(a.workspace), "%s: unaligned workspace", who);
   Params p = base_params(a);
   p.prefix = (int)std::min<int64_t>(a.prefix_len, 0x7FFFFFFF);
-  p.parts = plan.simt_parts;
   p.slots = plan.slots;
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)a.tokens * a.heads * plan.slots *
                                                        a.head_dim);
-  int rc = launch_simt(p, a.dtype, s);
-  if (!rc && plan.slots) rc = launch_join(p, a.dtype, s);
-  return rc;
+  if (plan.simt) {
+    p.parts = plan.simt_parts;
+    if (int rc = launch_simt(p, a.dtype, s)) return rc;
+  } else {
+    if (plan.prefix) {
+      Params shared = p;
+      shared.key_end = p.prefix;
+      if (int rc = launch_tiles(shared, a.dtype, true, plan.prefix_twin, plan.prefix_row_tiles,
+                                plan.prefix_parts, s))
+        return rc;
+      p.key_start = p.prefix;
+      p.slot0 = plan.prefix_parts * (plan.prefix_twin ? 2 : 1);
+    }
+    if (plan.decode) {
+      p.parts = plan.decode_parts;
+      if (int rc = launch_decode(p, a.dtype, plan.decode_per, s)) return rc;
+    } else if (int rc = launch_tiles(p, a.dtype, false, plan.twin, plan.row_tiles,
+                                     plan.tile_parts, s)) {
+      return rc;
+    }
+  }
+  return plan.slots ? launch_join(p, a.dtype, s) : IE_OK;
 }
 
 }  // namespace

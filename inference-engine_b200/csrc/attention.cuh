@@ -110,7 +110,19 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+constexpr int kSms = 148;
+
 // ---- launchers -------------------------------------------------------------
+// One token per sequence, 16-bit rows of 64 or 128 elements (attention_decode.cu);
+// part i of a row covers its visible keys [i * per, (i + 1) * per), the last one
+// to the end.
+int launch_decode(const Params& p, int dtype, int per, cudaStream_t s);
+// Rows in tiles on the tensor cores (attention_sm100.cu): every sequence's queries
+// over its own table, or (prefix) all queries over the first table row's keys below
+// key_end.  Part i writes slot slot0 + i, or, twin, slots slot0 + 2 i and 2 i + 1.
+int launch_tiles(const Params& p, int dtype, bool prefix, bool twin, int row_tiles, int parts,
+                 cudaStream_t s);
+uint32_t attention_status(bool clear);
 // Any type, head size up to 256 and alignment (attention_simt.cu).
 int launch_simt(const Params& p, int dtype, cudaStream_t s);
 // out = the joined parts [0, slots) of every row.

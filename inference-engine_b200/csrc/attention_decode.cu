@@ -1,0 +1,327 @@
+// Paged attention of one query token per sequence (decode), bf16 / f16 with heads
+// of 64 or 128 elements.
+//
+// Every key and value of a kv head is read once for all the query heads that
+// share it, so the kernel is bound by HBM: 4 flops per byte and query head,
+// far below the tensor cores' rate.  The query heads of a kv head form the 16
+// rows of an m16n8k16 product (more than 16 take several CTAs); its padded
+// rows cost tensor time that is idle anyway, and tcgen05's 128-row tile would
+// pad eight times more and keep the data path in shared memory and TMEM busy
+// for nothing.
+//
+// A CTA takes one part of one sequence's visible keys for one kv head.  Its four
+// warps work alone: a warp loads 16 keys and values at a time into its own
+// three-stage ring (cp.async, 16 bytes a lane, chunks XOR-swizzled by the row so
+// that ldmatrix is conflict-free), and keeps its own running maximum, sum and
+// output, joined at the end through shared memory.  No CTA barrier lies on the
+// path, two CTAs of an SM keep 128 KB of loads in flight, and pages of any size
+// cost one table lookup per key.
+//
+// The maximum is raised only when a score passes it by more than 2^8: the sums
+// stay far inside f32 and the outputs are rescaled a few times a row instead of
+// every step.  Weights are rounded to the element type for the product with
+// V, the rounding that the tensor cores' operands impose; their sum is not.
+#include "attention.cuh"
+
+namespace ie {
+namespace attn {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStep = 16;     // keys of a step
+constexpr int kStages = 3;
+constexpr float kLazy = 8.0f;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// 16 bytes, or zeros when !ok (the source is then not read)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4],
+                                                   uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                            uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int HD>
+constexpr int smem_bytes() {
+  return kWarps * kStages * kStep * HD * 2 * 2;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+attention_decode_kernel(const Params p, const int per) {
+  constexpr int kChunks = HD / 8;                 // 16-byte chunks of a row
+  constexpr int kRowBytes = HD * 2;
+  constexpr int kTile = kStep * kRowBytes;        // K or V of one stage
+  constexpr int kRowsAtOnce = 32 / kChunks;       // rows one warp-wide copy covers
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_ml[kWarps][16][2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row_groups = (p.group + 15) / 16;
+  int b = blockIdx.x;
+  const int part = b % p.parts;
+  b /= p.parts;
+  const int rg = b % row_groups;
+  b /= row_groups;
+  const int kvh = b % p.kv_heads;
+  const int seq = b / p.kv_heads;                 // also the query token
+  const Keys keys = keys_of(p, context_of(p, seq) - 1);
+  const int rows = min(16, p.group - rg * 16);
+  const int head0 = kvh * p.group + rg * 16;
+  const int k0 = (int)min((int64_t)part * per, (int64_t)keys.n);
+  const int k1 = part == p.parts - 1 ? keys.n : min(k0 + per, keys.n);
+  const int64_t row0 = (int64_t)seq * p.heads + head0;
+
+  if (k0 >= k1) {     // nothing of this row lies in this part
+    if (p.slots) {
+      if (threadIdx.x < rows)
+        p.part_ml[(row0 + threadIdx.x) * p.slots + p.slot0 + part] = make_float2(-INFINITY, 0.0f);
+    } else {
+      T* out = static_cast<T*>(p.out) + seq * p.out_token + (int64_t)head0 * HD;
+      for (int i = threadIdx.x; i < rows * HD; i += kWarps * 32) out[i] = from_f32<T>(0.0f);
+    }
+    return;
+  }
+
+  // ---- the query rows as A fragments
+  uint32_t qf[HD / 16][4];
+  {
+    const T* q = static_cast<const T*>(p.q) + seq * p.q_token + (int64_t)head0 * p.q_head;
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = lane / 4 + (i & 1) * 8, c = kk * 16 + (lane % 4) * 2 + (i >> 1) * 8;
+        qf[kk][i] = r < rows ? *reinterpret_cast<const uint32_t*>(q + r * p.q_head + c) : 0u;
+      }
+  }
+
+  const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * kTile);
+  const int32_t* table = p.tables + (int64_t)seq * p.table_stride;
+  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + (int64_t)kvh * p.head_stride * 2 +
+                         (lane % kChunks) * 16;
+  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + (int64_t)kvh * p.head_stride * 2 +
+                         (lane % kChunks) * 16;
+  const int64_t slot_bytes = p.slot_stride * 2;
+  const int steps = (k1 - k0 + kStep - 1) / kStep;
+  const int mine = (steps - warp + kWarps - 1) / kWarps;    // steps of this warp
+
+  // the cache row of key lane % 16 of this warp's step i (-1: not seen)
+  auto slot_of = [&](int i) {
+    const int key = k0 + (i * kWarps + warp) * kStep + (lane & 15);
+    return i < mine && key < k1 ? cache_slot(p, table, keys.at(key)) : -1;
+  };
+  auto load = [&](int i, int slot) {
+    const uint32_t dst = ring + (i % kStages) * (2 * kTile);
+#pragma unroll
+    for (int j = 0; j < kStep / kRowsAtOnce; ++j) {
+      const int r = j * kRowsAtOnce + lane / kChunks;
+      const int s = __shfl_sync(~0u, slot, r);
+      const uint32_t at = dst + r * kRowBytes + (((lane % kChunks) ^ (r & 7)) << 4);
+      const int64_t off = s < 0 ? 0 : s * slot_bytes;
+      cp_async16(at, kbase + off, s >= 0);
+      cp_async16(at + kTile, vbase + off, s >= 0);
+    }
+  };
+
+  float o[HD / 8][4] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  uint32_t seen[kStages];          // which of a stage's keys are there
+  int next = slot_of(0);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    seen[i] = __ballot_sync(~0u, next >= 0) & 0xFFFFu;
+    if (i < mine) load(i, next);
+    cp_commit();
+    next = slot_of(i + 1);
+  }
+  seen[kStages - 1] = 0;
+  for (int i = 0; i < mine; ++i) {
+    const int ahead = i + kStages - 1;
+    const uint32_t ahead_seen = __ballot_sync(~0u, next >= 0) & 0xFFFFu;
+    if (ahead < mine) load(ahead, next);
+    cp_commit();
+    next = slot_of(ahead + 1);
+    cp_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t kt = ring + (i % kStages) * (2 * kTile), vt = kt + kTile;
+    const uint32_t bits = seen[0];
+
+    float s[2][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk) {
+      const int r = (lane >> 4) * 8 + (lane & 7), c = kk * 2 + ((lane >> 3) & 1);
+      uint32_t f[4];
+      ldsm4(kt + r * kRowBytes + ((c ^ (r & 7)) << 4), f);
+      mma<T>(s[0], qf[kk], f[0], f[1]);
+      mma<T>(s[1], qf[kk], f[2], f[3]);
+    }
+    if (bits != 0xFFFFu) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!(bits >> (n * 8 + (lane % 4) * 2 + (e & 1)) & 1u)) s[n][e] = -INFINITY;
+    }
+    float mx[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 1));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 2)) * p.scale2;
+    }
+    if (__any_sync(~0u, mx[0] > m[0] + kLazy || mx[1] > m[1] + kLazy)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float mn = fmaxf(m[h], mx[h]);
+        const float f = mn == -INFINITY ? 1.0f : ex2(m[h] - mn);
+        m[h] = mn;
+        l[h] *= f;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          o[n][2 * h] *= f;
+          o[n][2 * h + 1] *= f;
+        }
+      }
+    }
+    uint32_t pf[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float w0 = ex2(fmaf(s[n][2 * h], p.scale2, -ref));
+        const float w1 = ex2(fmaf(s[n][2 * h + 1], p.scale2, -ref));
+        l[h] += w0 + w1;
+        const T t0 = from_f32<T>(w0), t1 = from_f32<T>(w1);
+        pf[n * 2 + h] = (uint32_t)*reinterpret_cast<const uint16_t*>(&t0) |
+                        (uint32_t)*reinterpret_cast<const uint16_t*>(&t1) << 16;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < HD / 16; ++n) {
+      const int r = ((lane >> 3) & 1) * 8 + (lane & 7), c = n * 2 + (lane >> 4);
+      uint32_t f[4];
+      ldsm4_trans(vt + r * kRowBytes + ((c ^ (r & 7)) << 4), f);
+      mma<T>(o[2 * n], pf, f[0], f[1]);
+      mma<T>(o[2 * n + 1], pf, f[2], f[3]);
+    }
+    __syncwarp();       // every lane has read the stage before it is loaded again
+#pragma unroll
+    for (int q = 0; q < kStages - 2; ++q) seen[q] = seen[q + 1];
+    seen[kStages - 2] = ahead_seen;
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(~0u, l[h], 1);
+    l[h] += __shfl_xor_sync(~0u, l[h], 2);
+  }
+
+  // ---- join the warps
+  __syncthreads();      // the rings are done with
+  float* s_o = reinterpret_cast<float*>(smem) + warp * (16 * HD);
+  if (lane % 4 == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s_ml[warp][lane / 4 + 8 * h][0] = m[h];
+      s_ml[warp][lane / 4 + 8 * h][1] = l[h];
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = lane / 4 + 8 * h;
+      if (r < rows)
+        *reinterpret_cast<float2*>(s_o + r * HD + n * 8 + (lane % 4) * 2) =
+            make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(smem);
+  for (int i = threadIdx.x; i < rows * (HD / 2); i += kWarps * 32) {
+    const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
+    float mt = s_ml[0][r][0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) mt = fmaxf(mt, s_ml[w][r][0]);
+    const float ref = mt == -INFINITY ? 0.0f : mt;
+    float lt = 0.0f, a = 0.0f, c = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(s_ml[w][r][0] - ref);
+      const float2 v = *reinterpret_cast<const float2*>(all + w * (16 * HD) + r * HD + d);
+      lt = fmaf(s_ml[w][r][1], f, lt);
+      a = fmaf(v.x, f, a);
+      c = fmaf(v.y, f, c);
+    }
+    if (p.slots) {
+      const int64_t at = (row0 + r) * p.slots + p.slot0 + part;
+      if (d == 0) p.part_ml[at] = make_float2(mt, lt);
+      *reinterpret_cast<float2*>(p.part_o + at * HD + d) = make_float2(a, c);
+    } else {
+      const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+      T* out = static_cast<T*>(p.out) + seq * p.out_token + (int64_t)(head0 + r) * HD + d;
+      out[0] = from_f32<T>(a * inv);
+      out[1] = from_f32<T>(c * inv);
+    }
+  }
+}
+
+template <typename T, int HD>
+int launch(const Params& p, int per, cudaStream_t s) {
+  auto kernel = attention_decode_kernel<T, HD>;
+  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   smem_bytes<HD>()));
+  const int64_t grid = (int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts;
+  kernel<<<(unsigned)grid, kWarps * 32, smem_bytes<HD>(), s>>>(p, per);
+  return launch_status("attention_decode_kernel");
+}
+
+}  // namespace
+
+int launch_decode(const Params& p, int dtype, int per, cudaStream_t s) {
+  if (dtype == IE_DT_BF16)
+    return p.hd == 64 ? launch<__nv_bfloat16, 64>(p, per, s) : launch<__nv_bfloat16, 128>(p, per, s);
+  return p.hd == 64 ? launch<__half, 64>(p, per, s) : launch<__half, 128>(p, per, s);
+}
+
+}  // namespace attn
+}  // namespace ie

@@ -9,6 +9,10 @@
 
 namespace ie {
 
+namespace attn {
+uint32_t attention_status(bool clear);   // attention_sm100.cu
+}
+
 namespace {
 thread_local char g_err[512] = "";
 }
@@ -132,7 +136,7 @@ extern "C" int ie_qlinear_noalloc(const ie_qlinear_args* a, void* stream) {
 
 extern "C" int ie_kernel_status(uint32_t* bits, int32_t clear) {
   IE_CHECK(bits, "kernel_status: null output");
-  *bits = tc_read_status(clear != 0);
+  *bits = tc_read_status(clear != 0) | attn::attention_status(clear != 0);
   return IE_OK;
 }
 

@@ -19,7 +19,8 @@ ROOT = PKG.parent                      # inference-engine_b200/
 CSRC = ROOT / "csrc"
 REPO = ROOT.parent
 SOURCES = ["capi.cu", "quant.cu", "gemv.cu", "qgemm_sm100.cu", "comm.cu", "norm.cu",
-           "rope_kv.cu", "attention.cu", "attention_simt.cu", "kv_pages.cu", "scoring.cu"]
+           "rope_kv.cu", "attention.cu", "attention_simt.cu", "attention_decode.cu",
+           "attention_sm100.cu", "kv_pages.cu", "scoring.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
