@@ -288,16 +288,16 @@ typedef struct ie_attention_args {
   int64_t max_query_len, max_context_len;   /* the longest of the batch (0: not known): they
                                                size the launch, any value gives the result */
   int64_t window, sinks, prefix_len;
-  void* workspace;                          /* ie_attention_workspace_size bytes, 16-byte
-                                               aligned, no initial contents; calls that
-                                               overlap on the GPU need their own */
-  size_t workspace_bytes;
   int32_t dtype, heads, kv_heads, head_dim, block_size;
-  float scale;                              /* of the scores, head_dim^-1/2 as a rule */
+  float scale;                              /* of the scores, > 0: head_dim^-1/2 as a rule */
 } ie_attention_args;
+/* workspace: ie_attention_workspace_size bytes (often 0), 16-byte aligned, no initial
+ * contents; calls that overlap on the GPU need their own. */
 size_t ie_attention_workspace_size(const ie_attention_args* a);
-int ie_window_attention(const ie_attention_args* a, void* stream);
-int ie_shared_prefix_attention(const ie_attention_args* a, void* stream);
+int ie_window_attention(const ie_attention_args* a, void* workspace, size_t workspace_bytes,
+                        void* stream);
+int ie_shared_prefix_attention(const ie_attention_args* a, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 /* ---- pages of the cache ------------------------------------------------------------
  * Page dst[i] <- page src[i] in each of `ncaches` caches (host array of device

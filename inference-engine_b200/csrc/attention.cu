@@ -104,22 +104,69 @@ struct Plan {
   int slots;                        // 0: a single part, written to out directly
 };
 
-// Parts of rows that see up to n keys, for `units` independent rows' worth of work
-// and `wide` CTAs at once: the fewest rounds of CTAs, where a CTA costs its
-// keys and `fixed` more (its start and end), and joining parts costs `join`.
+// Cost, in keys, of `units` independent rows' worth of n keys in `parts` parts, with
+// `wide` CTAs at once: the rounds of CTAs, where a CTA costs its keys (whole
+// steps) and `fixed` more (its start and end).
+int64_t rounds_cost(int64_t units, int64_t n, int64_t step, int64_t parts, int wide,
+                    int64_t fixed) {
+  return ceil_div(units * parts, wide) * (ceil_div(ceil_div(n, step), parts) * step + fixed);
+}
+
+// The cheapest number of parts, where joining them costs `join` + 4 a part.
 int best_parts(int64_t units, int64_t n, int64_t step, int wide, int64_t fixed, int64_t join) {
-  int64_t best = 1, least = -1;
-  const int64_t most = std::min<int64_t>(std::max<int64_t>(1, n / step), 128);
-  for (int64_t parts = 1; parts <= most; ++parts) {
-    const int64_t per = ceil_div(ceil_div(n, step), parts) * step;
-    const int64_t cost = ceil_div(units * parts, wide) * (per + fixed) +
-                         (parts > 1 ? join + 4 * parts : 0);
-    if (least < 0 || cost < least) {
+  int64_t best = 1, least = rounds_cost(units, n, step, 1, wide, fixed);
+  const int64_t most = std::min<int64_t>(n / step, 128);
+  for (int64_t parts = 2; parts <= most; ++parts) {
+    const int64_t cost = rounds_cost(units, n, step, parts, wide, fixed) + join + 4 * parts;
+    if (cost < least) {
       least = cost;
       best = parts;
     }
   }
   return (int)best;
+}
+
+// Parts of the decode kernel's rows and how they are joined.  Times are counted in
+// keys of one CTA of four warps (13 ns on B200 for heads of 128), fitted to
+// measurements over 1 to 64 sequences of 512 to 65536 keys:
+//   - 160 such CTAs draw all of HBM; a batch's contexts are taken to be 0.7 of the
+//     longest on average;
+//   - up to 148 CTAs have eight warps and take 0.65 of the time; the next 148 share
+//     SMs;
+//   - within one round of CTAs the longest part ends it (0.3 for uneven lengths),
+//     a second round that is short of half costs 0.6 of a CTA, and with more
+//     rounds the scheduler evens the lengths out (0.2);
+//   - a start costs 96, a join within a cluster 70, a joining launch 400 and 16 a
+//     part.
+void choose_decode(const ie_attention_args& a, int64_t units, int64_t own, Plan& plan) {
+  const double total = (a.seqs == 1 ? 1.0 : 0.7) * (double)(units * own) / 160;
+  auto cost = [&](int64_t parts) {
+    const int64_t ctas = units * parts;
+    const double cta = (double)(ceil_div(ceil_div(own, 64), parts) * 64 + 96) *
+                       (ctas <= kSms ? 0.65 : 1.0);
+    if (ctas <= 2 * kSms) return std::max(total, cta) + 0.3 * cta;
+    return total + (ctas < 3 * kSms ? 0.6 : 0.2) * cta;
+  };
+  const bool may_cluster = !plan.prefix;
+  double least = cost(1);
+  plan.decode_parts = 1;
+  plan.slots = plan.prefix ? 1 : 0;
+  const int64_t most = std::min<int64_t>(ceil_div(own, 64), 128);
+  for (int64_t parts = 2; parts <= most && units * parts <= 8 * kSms; ++parts) {
+    const double join = plan.prefix ? 16.0 * parts : 400.0 + 16.0 * parts;
+    if (cost(parts) + join < least) {
+      least = cost(parts) + join;
+      plan.decode_parts = plan.slots = (int)parts;
+    }
+  }
+  for (int parts = 2; may_cluster && parts <= kMaxDecodeCluster && units * parts <= 2 * kSms;
+       parts *= 2) {
+    if (cost(parts) + 70 <= least) {
+      least = cost(parts) + 70;
+      plan.decode_parts = parts;
+      plan.slots = 0;
+    }
+  }
 }
 
 Plan make_plan(const ie_attention_args& a) {
@@ -149,10 +196,8 @@ Plan make_plan(const ie_attention_args& a) {
   if (!a.cu_seqlens_q) {
     plan.decode = true;
     const int64_t units = a.seqs * a.kv_heads * ceil_div(group, 16);
-    // 64 keys of a CTA cost about what its start does, a join about 100
-    plan.decode_parts = best_parts(units, own, 64, 2 * kSms, 64, plan.prefix ? 0 : 100);
+    choose_decode(a, units, own, plan);
     plan.decode_per = (int)(ceil_div(ceil_div(own, 64), plan.decode_parts) * 64);
-    plan.slots = plan.decode_parts;
   } else {
     const int64_t queries = a.max_query_len > 0 ? std::min(a.max_query_len, a.tokens) : a.tokens;
     const int64_t rows = queries * group;
@@ -173,16 +218,17 @@ size_t part_bytes(const ie_attention_args& a, int slots) {
   return (size_t)a.tokens * a.heads * slots * (a.head_dim * 4 + 8);
 }
 
-int run(const ie_attention_args& a, const char* who, cudaStream_t s) {
+int run(const ie_attention_args& a, void* workspace, size_t workspace_bytes, const char* who,
+        cudaStream_t s) {
   const Plan plan = make_plan(a);
   const size_t need = part_bytes(a, plan.slots);
-  IE_CHECK(need == 0 || (a.workspace && a.workspace_bytes >= need),
-           "%s: a workspace of %zu bytes < %zu", who, a.workspace_bytes, need);
-  IE_CHECK(aligned16(a.workspace), "%s: unaligned workspace", who);
+  IE_CHECK(need == 0 || (workspace && workspace_bytes >= need),
+           "%s: a workspace of %zu bytes < %zu", who, workspace_bytes, need);
+  IE_CHECK(aligned16(workspace), "%s: unaligned workspace", who);
   Params p = base_params(a);
   p.prefix = (int)std::min<int64_t>(a.prefix_len, 0x7FFFFFFF);
   p.slots = plan.slots;
-  p.part_o = static_cast<float*>(a.workspace);
+  p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)a.tokens * a.heads * plan.slots *
                                                        a.head_dim);
   if (plan.simt) {
@@ -221,15 +267,17 @@ extern "C" size_t ie_attention_workspace_size(const ie_attention_args* a) {
   return part_bytes(*a, make_plan(*a).slots);
 }
 
-extern "C" int ie_window_attention(const ie_attention_args* a, void* stream) {
+extern "C" int ie_window_attention(const ie_attention_args* a, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
   IE_CHECK(a, "window_attention: null args");
   if (int rc = validate(*a, "window_attention")) return rc;
   IE_CHECK(a->prefix_len == 0, "window_attention: a shared prefix has its own entry point");
   if (a->tokens == 0) return IE_OK;
-  return run(*a, "window_attention", as_stream(stream));
+  return run(*a, workspace, workspace_bytes, "window_attention", as_stream(stream));
 }
 
-extern "C" int ie_shared_prefix_attention(const ie_attention_args* a, void* stream) {
+extern "C" int ie_shared_prefix_attention(const ie_attention_args* a, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
   IE_CHECK(a, "shared_prefix_attention: null args");
   if (int rc = validate(*a, "shared_prefix_attention")) return rc;
   IE_CHECK(a->window == 0 && a->sinks == 0,
@@ -238,5 +286,5 @@ extern "C" int ie_shared_prefix_attention(const ie_attention_args* a, void* stre
            "shared_prefix_attention: a prefix of %lld keys in tables of %lld",
            (long long)a->prefix_len, (long long)(a->table_width * a->block_size));
   if (a->tokens == 0) return IE_OK;
-  return run(*a, "shared_prefix_attention", as_stream(stream));
+  return run(*a, workspace, workspace_bytes, "shared_prefix_attention", as_stream(stream));
 }

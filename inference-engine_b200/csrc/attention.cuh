@@ -111,11 +111,12 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr int kSms = 148;
+constexpr int kMaxDecodeCluster = 8;
 
 // ---- launchers -------------------------------------------------------------
 // One token per sequence, 16-bit rows of 64 or 128 elements (attention_decode.cu);
 // part i of a row covers its visible keys [i * per, (i + 1) * per), the last one
-// to the end.
+// to the end.  Several parts without slots form clusters (at most 8 parts).
 int launch_decode(const Params& p, int dtype, int per, cudaStream_t s);
 // Rows in tiles on the tensor cores (attention_sm100.cu): every sequence's queries
 // over its own table, or (prefix) all queries over the first table row's keys below

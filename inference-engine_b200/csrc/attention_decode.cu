@@ -9,25 +9,30 @@
 // pad eight times more and keep the data path in shared memory and TMEM busy
 // for nothing.
 //
-// A CTA takes one part of one sequence's visible keys for one kv head.  Its four
+// A CTA takes one part of one sequence's visible keys for one kv head.  Its
 // warps work alone: a warp loads 16 keys and values at a time into its own
 // three-stage ring (cp.async, 16 bytes a lane, chunks XOR-swizzled by the row so
 // that ldmatrix is conflict-free), and keeps its own running maximum, sum and
 // output, joined at the end through shared memory.  No CTA barrier lies on the
-// path, two CTAs of an SM keep 128 KB of loads in flight, and pages of any size
-// cost one table lookup per key.
+// path, the eight warps of an SM (two CTAs of four or, where there are no more
+// CTAs than SMs, one of eight) keep 128 KB of loads in flight, and pages of any
+// size cost one table lookup per key.
 //
 // The maximum is raised only when a score passes it by more than 2^8: the sums
 // stay far inside f32 and the outputs are rescaled a few times a row instead of
 // every step.  Weights are rounded to the element type for the product with
 // V, the rounding that the tensor cores' operands impose; their sum is not.
+//
+// A few parts of a row form a thread-block cluster and are joined through
+// distributed shared memory: one launch, no workspace.
+#include <cooperative_groups.h>
+
 #include "attention.cuh"
 
 namespace ie {
 namespace attn {
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kStep = 16;     // keys of a step
 constexpr int kStages = 3;
 constexpr float kLazy = 8.0f;
@@ -80,13 +85,24 @@ __device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int HD>
+template <int HD, int kWarps>
 constexpr int smem_bytes() {
   return kWarps * kStages * kStep * HD * 2 * 2;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+// Two elements of a finished row.
+template <typename T>
+__device__ __forceinline__ void store(const Params& p, int t, int head, int hd, int d, float a,
+                                      float b, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(p.out) + t * p.out_token + (int64_t)head * hd + d;
+  out[0] = from_f32<T>(a * inv);
+  out[1] = from_f32<T>(b * inv);
+}
+
+// kCluster: the parts of a row are the CTAs of one cluster and join on their own.
+template <typename T, int HD, int kWarps, bool kCluster>
+__global__ void __launch_bounds__(kWarps * 32, 8 / kWarps)
 attention_decode_kernel(const Params p, const int per) {
   constexpr int kChunks = HD / 8;                 // 16-byte chunks of a row
   constexpr int kRowBytes = HD * 2;
@@ -94,6 +110,7 @@ attention_decode_kernel(const Params p, const int per) {
   constexpr int kRowsAtOnce = 32 / kChunks;       // rows one warp-wide copy covers
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_ml[kWarps][16][2];
+  __shared__ float2 s_part[16];      // (m, l) of this CTA's part
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row_groups = (p.group + 15) / 16;
   int b = blockIdx.x;
@@ -110,7 +127,7 @@ attention_decode_kernel(const Params p, const int per) {
   const int k1 = part == p.parts - 1 ? keys.n : min(k0 + per, keys.n);
   const int64_t row0 = (int64_t)seq * p.heads + head0;
 
-  if (k0 >= k1) {     // nothing of this row lies in this part
+  if (!kCluster && k0 >= k1) {     // nothing of this row lies in this part
     if (p.slots) {
       if (threadIdx.x < rows)
         p.part_ml[(row0 + threadIdx.x) * p.slots + p.slot0 + part] = make_float2(-INFINITY, 0.0f);
@@ -185,15 +202,20 @@ attention_decode_kernel(const Params p, const int per) {
     const uint32_t kt = ring + (i % kStages) * (2 * kTile), vt = kt + kTile;
     const uint32_t bits = seen[0];
 
-    float s[2][4] = {};
+    // two chains of products for each 8 keys: a dependent product waits for the last
+    float s[2][4] = {}, s2[2][4] = {};
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
       const int r = (lane >> 4) * 8 + (lane & 7), c = kk * 2 + ((lane >> 3) & 1);
       uint32_t f[4];
       ldsm4(kt + r * kRowBytes + ((c ^ (r & 7)) << 4), f);
-      mma<T>(s[0], qf[kk], f[0], f[1]);
-      mma<T>(s[1], qf[kk], f[2], f[3]);
+      mma<T>(kk & 1 ? s2[0] : s[0], qf[kk], f[0], f[1]);
+      mma<T>(kk & 1 ? s2[1] : s[1], qf[kk], f[2], f[3]);
     }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
     if (bits != 0xFFFFu) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -277,6 +299,7 @@ attention_decode_kernel(const Params p, const int per) {
     }
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(smem);
+  float* joined = reinterpret_cast<float*>(smem) + kWarps * 16 * HD;    // cluster: [16][HD]
   for (int i = threadIdx.x; i < rows * (HD / 2); i += kWarps * 32) {
     const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
     float mt = s_ml[0][r][0];
@@ -292,27 +315,72 @@ attention_decode_kernel(const Params p, const int per) {
       a = fmaf(v.x, f, a);
       c = fmaf(v.y, f, c);
     }
-    if (p.slots) {
+    if (kCluster) {
+      if (d == 0) s_part[r] = make_float2(mt, lt);
+      *reinterpret_cast<float2*>(joined + r * HD + d) = make_float2(a, c);
+    } else if (p.slots) {
       const int64_t at = (row0 + r) * p.slots + p.slot0 + part;
       if (d == 0) p.part_ml[at] = make_float2(mt, lt);
       *reinterpret_cast<float2*>(p.part_o + at * HD + d) = make_float2(a, c);
     } else {
-      const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-      T* out = static_cast<T*>(p.out) + seq * p.out_token + (int64_t)(head0 + r) * HD + d;
-      out[0] = from_f32<T>(a * inv);
-      out[1] = from_f32<T>(c * inv);
+      store<T>(p, seq, head0 + r, HD, d, a, c, lt);
     }
+  }
+  if (kCluster) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // each CTA joins its share of the elements, the parts in order
+    for (int i = part * (kWarps * 32) + threadIdx.x; i < rows * (HD / 2);
+         i += p.parts * (kWarps * 32)) {
+      const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
+      float mt = -INFINITY;
+      for (int q = 0; q < p.parts; ++q) mt = fmaxf(mt, cluster.map_shared_rank(s_part, q)[r].x);
+      const float ref = mt == -INFINITY ? 0.0f : mt;
+      float lt = 0.0f, a = 0.0f, c = 0.0f;
+      for (int q = 0; q < p.parts; ++q) {
+        const float2 x = cluster.map_shared_rank(s_part, q)[r];
+        const float2 v = *reinterpret_cast<const float2*>(
+            cluster.map_shared_rank(joined, q) + r * HD + d);
+        const float f = ex2(x.x - ref);
+        lt = fmaf(x.y, f, lt);
+        a = fmaf(v.x, f, a);
+        c = fmaf(v.y, f, c);
+      }
+      store<T>(p, seq, head0 + r, HD, d, a, c, lt);
+    }
+    cluster.sync();      // the others have read this CTA's part
   }
 }
 
+template <typename T, int HD, int kWarps, bool kCluster>
+int launch(const Params& p, int per, cudaStream_t s) {
+  auto kernel = attention_decode_kernel<T, HD, kWarps, kCluster>;
+  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   smem_bytes<HD, kWarps>()));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem_bytes<HD, kWarps>();
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  if (kCluster) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+  }
+  IE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, per));
+  return IE_OK;
+}
 template <typename T, int HD>
 int launch(const Params& p, int per, cudaStream_t s) {
-  auto kernel = attention_decode_kernel<T, HD>;
-  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   smem_bytes<HD>()));
-  const int64_t grid = (int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts;
-  kernel<<<(unsigned)grid, kWarps * 32, smem_bytes<HD>(), s>>>(p, per);
-  return launch_status("attention_decode_kernel");
+  const bool cluster = p.parts > 1 && p.slots == 0;
+  const int64_t ctas = (int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts;
+  if (ctas <= kSms)
+    return cluster ? launch<T, HD, 8, true>(p, per, s) : launch<T, HD, 8, false>(p, per, s);
+  return cluster ? launch<T, HD, 4, true>(p, per, s) : launch<T, HD, 4, false>(p, per, s);
 }
 
 }  // namespace

@@ -124,8 +124,6 @@ class AttentionArgs(ctypes.Structure):
         ("window", ctypes.c_int64),
         ("sinks", ctypes.c_int64),
         ("prefix_len", ctypes.c_int64),
-        ("workspace", ctypes.c_void_p),
-        ("workspace_bytes", ctypes.c_size_t),
         ("dtype", ctypes.c_int32),
         ("heads", ctypes.c_int32),
         ("kv_heads", ctypes.c_int32),
@@ -162,8 +160,10 @@ def _declare(lib: ctypes.CDLL) -> None:
         "ie_rope_kv": (ctypes.c_int, [_P, _I64, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _I64,
                                       _I32, _P, _P, _P, _I64, _P, _P]),
         "ie_attention_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
-        "ie_window_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _P]),
-        "ie_shared_prefix_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _P]),
+        "ie_window_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _P,
+                                               ctypes.c_size_t, _P]),
+        "ie_shared_prefix_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _P,
+                                                      ctypes.c_size_t, _P]),
         "ie_copy_pages": (ctypes.c_int, [ctypes.POINTER(_P), _I32, _I64, _I64, _P, _P, _I64,
                                          _P]),
         "ie_token_logprobs": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _P, _I32, _P, _P, _P,
@@ -235,7 +235,24 @@ def check(code: int, what: str = "") -> None:
 
 def stream_ptr(stream=None) -> int | None:
     """Raw cudaStream_t of a torch stream (the current one when None)."""
+    if stream is not None:
+        return stream.cuda_stream or None
+    return _current_raw_stream() or None
+
+
+def _find_raw_stream():
+    """The current stream's address without making a Stream object (3 us a call)
+    where this torch has the call for it."""
     import torch
 
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream or None
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    device = getattr(torch._C, "_cuda_getDevice", None)
+    if raw is None or device is None:
+        return lambda: torch.cuda.current_stream().cuda_stream
+    return lambda: raw(device())
+
+
+def _current_raw_stream() -> int:
+    global _current_raw_stream
+    _current_raw_stream = _find_raw_stream()
+    return _current_raw_stream()

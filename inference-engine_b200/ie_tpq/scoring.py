@@ -4,15 +4,19 @@ from __future__ import annotations
 
 from typing import NamedTuple
 
+import torch
+
 from . import _lib
 from .device import dtype_code, require_cuda
 
+_READY = False
+
 
 class TokenLogprobs(NamedTuple):
-    logprobs: "torch.Tensor"        # f32 [rows]
-    entropy: "torch.Tensor"         # f32 [rows], nats
-    top_logprobs: "torch.Tensor"    # f32 [rows, top], best first
-    top_tokens: "torch.Tensor"      # int64 [rows, top], ties to the lower token
+    logprobs: torch.Tensor        # f32 [rows]
+    entropy: torch.Tensor         # f32 [rows], nats
+    top_logprobs: torch.Tensor    # f32 [rows, top], best first
+    top_tokens: torch.Tensor      # int64 [rows, top], ties to the lower token
 
 
 def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
@@ -24,7 +28,10 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     Logits of -inf (a vocabulary mask) are allowed; a row with a NaN or +inf, or
     with no logit above -inf, gives NaN.
     """
-    torch = require_cuda()
+    global _READY
+    if not _READY:
+        require_cuda()
+        _READY = True
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be a row-contiguous 2-D tensor")
     rows, vocab = logits.shape
@@ -41,12 +48,15 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     if stream is not None and stream != torch.cuda.current_stream():
         with torch.cuda.stream(stream):   # the outputs belong to that stream
             return token_logprobs(logits, tokens, top)
-    device = logits.device
-    both = torch.empty((2, rows), dtype=torch.float32, device=device)
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
-    top_tokens = torch.empty((rows, top), dtype=torch.long, device=device)
-    _lib.check(_lib.lib().ie_token_logprobs(
+    f32, device = torch.float32, logits.device
+    logprobs = torch.empty(rows, dtype=f32, device=device)
+    entropy = torch.empty(rows, dtype=f32, device=device)
+    top_logprobs = torch.empty(rows, top, dtype=f32, device=device)
+    top_tokens = torch.empty(rows, top, dtype=torch.long, device=device)
+    code = _lib.lib().ie_token_logprobs(
         logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), rows, vocab,
-        tokens.data_ptr(), top, both.data_ptr(), both.data_ptr() + 4 * rows,
-        top_logprobs.data_ptr(), top_tokens.data_ptr(), _lib.stream_ptr()), "token_logprobs")
-    return TokenLogprobs(both[0], both[1], top_logprobs, top_tokens)
+        tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(),
+        top_logprobs.data_ptr(), top_tokens.data_ptr(), _lib.stream_ptr())
+    if code:
+        _lib.check(code, "token_logprobs")
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

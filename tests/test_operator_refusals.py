@@ -29,13 +29,14 @@ def args(**kw):
     dict(tokens=-1), dict(tokens=3), dict(seqs=1), dict(seqs=-1), dict(block_size=0),
     dict(table_width=1 << 30), dict(table_width=-1), dict(cache_slots=-1),
     dict(cache_slots=1 << 31), dict(window=-1), dict(sinks=-1), dict(max_query_len=-1),
-    dict(max_context_len=-1), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=None),
+    dict(max_context_len=-1), dict(scale=float("inf")),
+    dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(q=None),
     dict(out=None), dict(block_tables=None), dict(context_lens=None), dict(k_cache=None),
     dict(q=4097), dict(v_cache=4097), dict(out_token_stride=100), dict(prefix_len=1),
     dict(tokens=0, seqs=0, cu_seqlens_q=4096, window=-5)])
 def test_window_attention(kw):
     a = args(**kw)
-    assert _lib.lib().ie_window_attention(ctypes.byref(a), None) == _lib.IE_ERR_INVALID
+    assert _lib.lib().ie_window_attention(ctypes.byref(a), None, 0, None) == _lib.IE_ERR_INVALID
     assert _lib.last_error().startswith("window_attention")
 
 
@@ -43,28 +44,27 @@ def test_window_attention(kw):
                                 dict(prefix_len=-1), dict(heads=3)])
 def test_shared_prefix_attention(kw):
     a = args(**kw)
-    assert _lib.lib().ie_shared_prefix_attention(ctypes.byref(a), None) == _lib.IE_ERR_INVALID
+    assert _lib.lib().ie_shared_prefix_attention(ctypes.byref(a), None, 0, None) == _lib.IE_ERR_INVALID
     assert _lib.last_error().startswith("shared_prefix_attention")
 
 
 def test_workspace_that_is_missing_or_small():
     lib = _lib.lib()
-    for a, entry in ((args(table_width=4096), lib.ie_window_attention),
+    for a, entry in ((args(table_width=1 << 16), lib.ie_window_attention),
                      (args(table_width=4096, prefix_len=4096), lib.ie_shared_prefix_attention)):
         need = lib.ie_attention_workspace_size(ctypes.byref(a))
         assert need > 0
-        assert entry(ctypes.byref(a), None) == _lib.IE_ERR_INVALID
-        a.workspace, a.workspace_bytes = 4096, need - 1
-        assert entry(ctypes.byref(a), None) == _lib.IE_ERR_INVALID
+        for at, size in ((None, 0), (None, need), (4096, need - 1), (4104, need)):
+            assert entry(ctypes.byref(a), at, size, None) == _lib.IE_ERR_INVALID
     assert lib.ie_attention_workspace_size(None) == 0
     assert lib.ie_attention_workspace_size(ctypes.byref(args(heads=3))) == 0
-    assert lib.ie_window_attention(None, None) == _lib.IE_ERR_INVALID
+    assert lib.ie_window_attention(None, None, 0, None) == _lib.IE_ERR_INVALID
 
 
 def test_nothing_to_do_is_not_an_error():
     a = args(tokens=0, seqs=0)
-    assert _lib.lib().ie_window_attention(ctypes.byref(a), None) == _lib.IE_OK
-    assert _lib.lib().ie_shared_prefix_attention(ctypes.byref(a), None) == _lib.IE_OK
+    assert _lib.lib().ie_window_attention(ctypes.byref(a), None, 0, None) == _lib.IE_OK
+    assert _lib.lib().ie_shared_prefix_attention(ctypes.byref(a), None, 0, None) == _lib.IE_OK
     assert _lib.lib().ie_copy_pages(None, 0, 16, 4, None, None, 0, None) == _lib.IE_OK
     assert _lib.lib().ie_token_logprobs(None, 8, 2, 0, 8, None, 0, None, None, None, None,
                                         None) == _lib.IE_OK
