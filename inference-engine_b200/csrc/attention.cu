@@ -71,6 +71,7 @@ Params base_params(const ie_attention_args& a) {
   p.hd = a.head_dim;
   p.table_width = (int)a.table_width;
   p.pages = (int)(a.cache_slots / a.block_size);
+  p.cache_rows = (int)a.cache_slots;
   p.block = FastDiv((uint32_t)a.block_size);
   p.group_div = FastDiv((uint32_t)p.group);
   const int64_t most = 1 << 30;
@@ -175,7 +176,9 @@ Plan make_plan(const ie_attention_args& a) {
   int64_t keys = a.table_width * a.block_size;      // of the longest context
   if (a.max_context_len > 0) keys = std::min(keys, a.max_context_len);
   const int64_t seen = a.window > 0 ? std::min(keys, a.window + a.sinks) : keys;
-  if (!tensor_cores(a)) {
+  const int64_t per_tile = 128 / group;     // tokens of a row tile of the tensor cores
+  // (a group of more than 128 heads has only the decode kernel)
+  if (!tensor_cores(a) || (per_tile == 0 && (a.cu_seqlens_q || a.prefix_len > 0))) {
     // enough CTAs for every SM's warps, at least 64 keys each
     plan.simt = true;
     const int64_t rows = a.tokens * a.heads;
@@ -186,9 +189,8 @@ Plan make_plan(const ie_attention_args& a) {
   }
   plan.prefix = a.prefix_len > 0;
   if (plan.prefix) {
-    const int64_t rows = a.tokens * group;
-    plan.prefix_twin = rows <= 128;
-    plan.prefix_row_tiles = (int)ceil_div(rows, plan.prefix_twin ? 128 : 256);
+    plan.prefix_twin = a.tokens <= per_tile;
+    plan.prefix_row_tiles = (int)ceil_div(a.tokens, plan.prefix_twin ? per_tile : 2 * per_tile);
     plan.prefix_parts = best_parts(plan.prefix_row_tiles * a.kv_heads, a.prefix_len, 128, kSms,
                                    256, 512);
   }
@@ -200,11 +202,10 @@ Plan make_plan(const ie_attention_args& a) {
     plan.decode_per = (int)(ceil_div(ceil_div(own, 64), plan.decode_parts) * 64);
   } else {
     const int64_t queries = a.max_query_len > 0 ? std::min(a.max_query_len, a.tokens) : a.tokens;
-    const int64_t rows = queries * group;
-    plan.twin = rows <= 128 && own > 128;
-    plan.row_tiles = (int)ceil_div(rows, plan.twin ? 128 : 256);
+    plan.twin = queries <= per_tile && own > 128;
+    plan.row_tiles = (int)ceil_div(queries, plan.twin ? per_tile : 2 * per_tile);
     // a row tile sees the window of its first token and what lies up to its last
-    const int64_t n = a.window > 0 ? std::min(own, seen + ceil_div(256, group)) : own;
+    const int64_t n = a.window > 0 ? std::min(own, seen + 2 * per_tile) : own;
     plan.tile_parts = best_parts(plan.row_tiles * a.seqs * a.kv_heads, n, 128, kSms, 256,
                                  plan.prefix ? 0 : 512);
     plan.slots = plan.tile_parts * (plan.twin ? 2 : 1);

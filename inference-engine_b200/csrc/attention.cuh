@@ -36,7 +36,7 @@ struct Params {
   const int32_t* context;
   const int32_t* cu_q;            // null: one token per sequence
   int tokens, seqs, heads, kv_heads, group, hd;
-  int table_width, pages;
+  int table_width, pages, cache_rows;   // rows: slots of the cache
   FastDiv block, group_div;
   int window, sinks;              // window 0: every earlier key
   int prefix;                     // keys below it are looked up in the first table row

@@ -35,11 +35,15 @@
 //
 // A key that some rows of a tile see and others do not enters the others'
 // product with weight 0; a NaN or infinite V there would still poison them.  Rows
-// that come out not finite are therefore computed again key by key, leaving out what
-// they do not see.
+// that come out not finite although their weights are finite are therefore computed
+// again key by key, leaving out what they do not see.
 //
 // Every wait has a limit; a wait that runs out sets an error bit
 // (ie_kernel_status) and all roles leave.
+#include <cuda.h>
+
+#include <mutex>
+
 #include "attention.cuh"
 
 namespace ie {
@@ -47,9 +51,12 @@ namespace attn {
 namespace {
 
 constexpr int kTile = 128;         // rows of a row tile, keys of a key tile
-constexpr int kThreads = 512;
-constexpr int kLoaders = 128;
+constexpr int kLoaders = 128;      // threads that gather K and V rows
+constexpr int kQLoaders = 64;      // threads that load the query rows
 constexpr float kLazy = 8.0f;
+// Rows of a TMA box.  Boxes of 16 rows leave the tensor cores waiting (490 us against 440 for
+// 2 x 8192 tokens, window 2048); larger ones than 32 only add masked keys to the window.
+constexpr int kMaxBox = 32;
 constexpr long long kWaitCycles = 4000000000ll;   // ~2 s
 constexpr int kInvalidRing = 8;
 
@@ -57,13 +64,31 @@ __device__ uint32_t g_attention_status = 0;
 
 enum Mode { kPrefill = 0, kPrefix = 1 };
 
+// Warps: 0-7 softmax, then the loaders of K and V (one warp with TMA, four that
+// gather), the issuing warp and two that load the query rows.
+template <bool kTma> struct Warps {
+  static constexpr int kIssue = kTma ? 9 : 12, kQuery = kIssue + 1;
+  static constexpr int kThreads = kTma ? 384 : 512;
+  // registers of the softmax warps and of the others: together the launch's
+  // (384 x 168: 256 x 208 + 128 x 88; 512 x 128: 256 x 192 + 256 x 64)
+  static constexpr int kSoftmaxRegs = kTma ? 208 : 192, kOtherRegs = kTma ? 88 : 64;
+};
+
 struct TileParams {
   Params p;
+  int box;           // rows of a TMA box (0: K and V are gathered)
   int mode;
   int twin;          // one row tile, two streams of key tiles
-  int row_tiles;     // work tiles (256 rows, or 128 when twin) of a segment in the grid
+  int per_tile;      // tokens of a row tile: 128 / group
+  int row_tiles;     // work tiles (two row tiles, one when twin) of a segment in the grid
+  bool wide_out;     // out rows are 32-byte aligned
   int segs;          // sequences (prefill) or 1 (prefix)
   int parts;         // key parts of a work tile
+};
+
+struct Maps {
+  CUtensorMap map[4];   // K, V in boxes; K, V row by row
+  CUtensorMap q;
 };
 
 // ---- PTX ---------------------------------------------------------------------
@@ -105,10 +130,42 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* quit) {
   return __all_sync(~0u, mbar_wait(bar, parity, quit));
 }
+// True in one lane of a converged warp.  The instructions of the asynchronous units take
+// their operands from uniform registers: a whole warp runs the code around them
+// (so that the compiler keeps the operands there) and one lane issues.
+__device__ __forceinline__ bool elect() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)::"memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(ok ? 16 : 0)
                : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                          int z, int u, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(u), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -124,27 +181,33 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       bool accumulate) {
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          bar),
+      "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       bool accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b,
+                                       uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b,
+                                       uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
 // 64 consecutive columns of this thread's lane; the registers are defined once
@@ -198,9 +261,13 @@ __device__ __forceinline__ void tmem_st_wait() {
 // groups of 8 rows 1024 bytes apart (SBO; LBO unused).  MN-major (V): 64 elements
 // along the head are adjacent, groups of 8 keys 1024 bytes apart (SBO), the next
 // 64 elements 16384 bytes on (LBO).
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
+// The low word (address in 16-byte units, LBO above it) moves with the start address.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+  return ((lbo >> 4) << 16) | ((addr & 0x3FFFFu) >> 4);
+}
+__device__ __forceinline__ uint64_t desc(uint32_t lo) {
   constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-  return ((uint64_t)hi << 32) | ((lbo >> 4) << 16) | ((addr & 0x3FFFFu) >> 4);
+  return ((uint64_t)hi << 32) | lo;
 }
 // f32 accumulator, A and B of type T, M = 128, N = n; B MN-major or not.
 template <typename T>
@@ -234,7 +301,7 @@ struct Layout {
   static constexpr int kBytes = kControl + 2048 + 1024;   // + alignment of the base
 };
 struct Control {
-  uint64_t full[8], empty[8], s_full[2], p_ready[2], o_done[2], q_free;
+  uint64_t full[8], empty[8], s_full[2], p_ready[2], o_done[2], q_full, q_free;
   int slots[2][kTile];                     // cache rows of a key tile
   alignas(16) uint32_t invalid[kInvalidRing][4];   // keys of a tile whose page is not there
   uint32_t tmem;
@@ -243,16 +310,23 @@ struct Control {
 static_assert(sizeof(Control) <= 2048, "control block");
 
 // ---- work ------------------------------------------------------------------------
-// One work tile: rows [row0, row0 + 256 or 128) of a segment for one kv head, and the
-// key tiles [j0, j1) of its virtual keys.  Every role derives it alike.
+// One work tile: the tokens from `first` on of a segment (two row tiles of
+// per_tile tokens, one when twin) for one kv head, and the key tiles [j0, j1) of
+// its virtual keys.  Every role derives it alike.
 struct Work {
-  int seg, kvh, part, row0, nrows;     // nrows: rows of the segment
-  int tok0, ctx, ntok;                 // first token, context, tokens (prefill)
+  int seg, kvh, part, first;
+  int tok0, ctx, ntok;                 // of the segment: first token, context, tokens
   int lo, ns, n;                       // virtual keys: ns sinks, then from lo
   int j0, j1;
 };
 
-__device__ __forceinline__ int rows_of_work(const TileParams& a) { return a.twin ? 128 : 256; }
+__device__ __forceinline__ int tokens_of_work(const TileParams& a) {
+  return a.twin ? a.per_tile : 2 * a.per_tile;
+}
+// row tiles of the work tile that hold tokens
+__device__ __forceinline__ int row_tiles_of(const TileParams& a, const Work& w) {
+  return !a.twin && w.ntok - w.first > a.per_tile ? 2 : 1;
+}
 
 // Segment of work item `item` and its first work tile; false: nothing there.
 __device__ __forceinline__ bool segment(const TileParams& a, int item, Work& w, int& tile) {
@@ -275,22 +349,24 @@ __device__ __forceinline__ bool segment(const TileParams& a, int item, Work& w, 
     w.ntok = min(w.ntok, p.tokens - w.tok0);
     w.ctx = context_of(p, w.seg);
   }
-  w.nrows = w.ntok * p.group;
-  return w.nrows > tile * rows_of_work(a);
+  return w.ntok > tile * tokens_of_work(a);
 }
 __device__ __forceinline__ void locate(const TileParams& a, Work& w, int tile) {
   const Params& p = a.p;
-  w.row0 = tile * rows_of_work(a);
+  w.first = tile * tokens_of_work(a);
   if (a.mode == kPrefix) {
     w.lo = w.ns = 0;
     w.n = p.key_end;
   } else {
-    const int t0 = p.group_div.div(w.row0);
-    const int t1 = p.group_div.div(min(w.row0 + rows_of_work(a), w.nrows) - 1);
-    const int first = max(w.ctx - w.ntok + t0, 0), last = w.ctx - w.ntok + t1;
+    const int first = max(w.ctx - w.ntok + w.first, 0);
+    const int last = w.ctx - w.ntok + min(w.first + tokens_of_work(a), w.ntok) - 1;
     w.lo = p.key_start;
     if (p.window > 0) w.lo = max(w.lo, first - p.window + 1);
     w.ns = p.key_start == 0 ? min(p.sinks, w.lo) : 0;
+    if (a.box > 1) {        // whole boxes: what they add is masked
+      w.lo &= ~(a.box - 1);
+      w.ns = min((w.ns + a.box - 1) & ~(a.box - 1), w.lo);
+    }
     const int hi = min(last + 1, p.key_end);
     w.n = last < 0 ? 0 : w.ns + max(hi - w.lo, 0);
   }
@@ -323,7 +399,9 @@ __device__ __noinline__ void row_again(const TileParams& a, const Work& w, int t
     if (a.twin && ((j - w.j0) & 1) != stream) continue;
     for (int v = j * kTile; v < min((j + 1) * kTile, w.n); ++v) {
       const int key = v < w.ns ? v : w.lo + v - w.ns;
-      if (key > pos || !(p.window == 0 || key > pos - p.window || key < p.sinks)) continue;
+      if (key > pos || key < p.key_start ||
+          !(p.window == 0 || key > pos - p.window || key < p.sinks))
+        continue;
       const int slot = cache_slot(p, table, key);
       if (slot < 0) continue;
       const int64_t at = slot * p.slot_stride + lane;
@@ -345,9 +423,25 @@ __device__ __noinline__ void row_again(const TileParams& a, const Work& w, int t
   *l_out = l;
 }
 
+// 32 bytes of a thread's own row: a whole sector a store where the row allows it
+__device__ __forceinline__ void store32(void* at, const uint32_t* x, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(x[0]),
+                 "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                 : "memory");
+  } else {
+    static_cast<uint4*>(at)[0] = make_uint4(x[0], x[1], x[2], x[3]);
+    static_cast<uint4*>(at)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+  }
+}
+// bits 0 .. n-1
+__device__ __forceinline__ uint32_t below(int n) {
+  return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
 // ---- roles ---------------------------------------------------------------------------
 template <typename T, int HD>
-__device__ void load_role(const TileParams& a, uint8_t* base, Control* c, int items) {
+__device__ void gather_role(const TileParams& a, uint8_t* base, Control* c, int items) {
   using L = Layout<HD>;
   const Params& p = a.p;
   constexpr int kChunks = HD / 8;                  // 16-byte chunks of a row
@@ -362,7 +456,6 @@ __device__ void load_role(const TileParams& a, uint8_t* base, Control* c, int it
   const int64_t slot_bytes = p.slot_stride * 2;
   uint32_t item = 0;          // stages filled so far (K and V tiles alternate)
   uint32_t told = 0;          // stages whose arrival is done
-  uint32_t qn = 0;            // work tiles loaded
   bool failed = false;        // a wait of this thread ran out
 
   // Barrier of the loaders that tells all of them whether any has failed, so that they
@@ -415,7 +508,7 @@ __device__ void load_role(const TileParams& a, uint8_t* base, Control* c, int it
                         chunk * 16;
     const uint8_t* vb = static_cast<const uint8_t*>(p.v) + (int64_t)w.kvh * p.head_stride * 2 +
                         chunk * 16;
-    for (; tile * rows_of_work(a) < w.nrows; tile += a.row_tiles) {
+    for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
       if (w.j0 >= w.j1) continue;
       auto slot_at = [&](int j) {
@@ -424,27 +517,6 @@ __device__ void load_role(const TileParams& a, uint8_t* base, Control* c, int it
         return cache_slot(p, table, v < w.ns ? v : w.lo + v - w.ns);
       };
       int next = slot_at(w.j0);
-      // the query rows; their arrival is that of the first K tile
-      if (qn > 0) {
-        const uint32_t bar = smem_u32(&c->q_free), parity = (qn - 1) & 1;
-        if (!mbar_try(bar, parity)) {
-          flush();
-          failed = !mbar_wait(bar, parity, &c->quit);
-        }
-      }
-      ++qn;
-      const uint8_t* qb = static_cast<const uint8_t*>(p.q) + chunk * 16;
-      for (int i = 0; i < rows_of_work(a) / kRows; ++i) {
-        const int r = r0 + i * kRows, row = w.row0 + r;
-        const bool ok = row < w.nrows;
-        const int tok = ok ? p.group_div.div(row) : 0;
-        const int g = ok ? row - tok * p.group : 0;
-        const uint8_t* src = qb + ((w.tok0 + tok) * p.q_token +
-                                   (int64_t)(w.kvh * p.group + g) * p.q_head) * 2;
-        cp_async16(smem_u32(base + L::kQ) + (r / kTile) * L::kTileBytes + lane_off +
-                       (i * kRows % kTile) * 128,
-                   ok ? src : qb, ok);
-      }
       for (int j = w.j0; j < w.j1; ++j) {
         const uint32_t n = item / 2;      // key tiles before this one
         int* slots = c->slots[n & 1];
@@ -472,93 +544,275 @@ __device__ void load_role(const TileParams& a, uint8_t* base, Control* c, int it
   flush();
 }
 
+// One warp loads K and V with TMA: boxes of a.box rows (a power of two that divides
+// the page, so a box lies in one page) by 64 elements.  Lane g looks up box g of the
+// tile, one lane issues them all.  A box whose page is not there, and rows past the
+// last key, are read outside the tensor: zeros.
 template <typename T, int HD>
-__device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int items,
-                           uint32_t tmem) {
+__device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* base, Control* c,
+                         int items) {
   using L = Layout<HD>;
-  const uint32_t q0 = smem_u32(base + L::kQ), ring = smem_u32(base + L::kRing);
-  constexpr uint32_t kIdS = idesc<T>(kTile, false), kIdO = idesc<T>(HD, true);
-  uint32_t item = 0;                  // stages consumed by finished work tiles
-  uint32_t np[2] = {0, 0};            // p_ready phases waited for
-
-  auto full = [&](uint32_t i) {
-    return mbar_wait(smem_u32(&c->full[i % L::kStages]), (i / L::kStages) & 1, &c->quit);
-  };
-  auto p_ready = [&](int s) {
-    const bool ok = mbar_wait(smem_u32(&c->p_ready[s]), np[s] & 1, &c->quit);
-    ++np[s];
-    return ok;
-  };
-  auto scores = [&](int s, int q, uint32_t i) {      // S_s = Q_q K_i^T
-    const uint32_t k = ring + (i % L::kStages) * L::kTileBytes;
-#pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk) {
-      const uint32_t off = (kk / 4) * 16384 + (kk % 4) * 32;
-      mma_ss(tmem + s * kTile, desc(q0 + q * L::kTileBytes + off, 16), desc(k + off, 16), kIdS,
-             kk > 0);
-    }
-    tc_commit(smem_u32(&c->s_full[s]));
-  };
-  auto product = [&](int s, uint32_t i, bool first) {   // O_s (+)= P_s V_i
-    const uint32_t v = ring + (i % L::kStages) * L::kTileBytes;
-#pragma unroll
-    for (int kk = 0; kk < kTile / 16; ++kk)
-      mma_ts(tmem + 2 * kTile + s * HD, tmem + s * kTile + kk * 8, desc(v + kk * 2048, 16384),
-             kIdO, !first || kk > 0);
-  };
-  auto release = [&](uint32_t i) { tc_commit(smem_u32(&c->empty[i % L::kStages])); };
+  const Params& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int groups = kTile / a.box;
+  const int v_lane = lane * a.box;         // this lane's box, if lane < groups
+  const uint32_t ring = smem_u32(base + L::kRing);
+  const int outside = p.cache_rows;
+  uint32_t item = 0;
 
   for (int it = blockIdx.x; it < items; it += gridDim.x) {
     Work w;
     int tile;
     if (!segment(a, it, w, tile)) continue;
-    for (; tile * rows_of_work(a) < w.nrows; tile += a.row_tiles) {
+    const int32_t* table = p.tables + (a.mode == kPrefix ? 0 : (int64_t)w.seg * p.table_stride);
+    for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
+      locate(a, w, tile);
+      // cache row of this lane's box of key tile j: -1 no page, -2 no key
+      auto row_at = [&](int j) {
+        const int v = j * kTile + v_lane;
+        if (lane >= groups || j >= w.j1 || v >= w.n) return -2;
+        return cache_slot(p, table, v < w.ns ? v : w.lo + v - w.ns);
+      };
+      int next = row_at(w.j0);
+      for (int j = w.j0; j < w.j1; ++j) {
+        const int row = next;
+        next = row_at(j + 1);
+        const uint32_t n = item / 2;      // key tiles before this one
+        const bool bad = row == -1;
+        uint32_t words[4] = {0u, 0u, 0u, 0u};
+        if (__any_sync(~0u, bad)) {
+          const int bit = v_lane;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            words[i] = __reduce_or_sync(
+                ~0u, bad && bit / 32 == i ? below(a.box) << (bit % 32) : 0u);
+        }
+        // boxes that end past the last key are read row by row
+        const int rows = row < 0 ? 0 : min(w.n - (j * kTile + v_lane), a.box);
+        const uint32_t ragged = __ballot_sync(~0u, rows > 0 && rows < a.box);
+        const int at = rows > 0 ? row : outside;
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t st = item % L::kStages, bar = smem_u32(&c->full[st]);
+          if (item >= L::kStages &&
+              !warp_wait(smem_u32(&c->empty[st]), (item / L::kStages - 1) & 1, &c->quit)) {
+            // what has been started ends before the CTA does
+            const long long t0 = clock64();
+            for (uint32_t i = item - L::kStages; i != item; ++i)
+              while (!mbar_try(smem_u32(&c->full[i % L::kStages]), (i / L::kStages) & 1) &&
+                     clock64() - t0 < kWaitCycles) {
+              }
+            return;
+          }
+          if (lane == 0) {
+            if (kv == 0)
+              *reinterpret_cast<uint4*>(c->invalid[n % kInvalidRing]) =
+                  make_uint4(words[0], words[1], words[2], words[3]);
+            mbar_expect(bar, L::kTileBytes);
+          }
+          __syncwarp();
+          const uint32_t dst = ring + st * L::kTileBytes;
+#pragma unroll 8
+          for (int g = 0; g < groups; ++g) {
+            const int y = __shfl_sync(~0u, at, g);
+            const int skip = ragged >> g & 1;
+            if (elect()) {
+#pragma unroll
+              for (int h = 0; h < L::kHalves; ++h)
+                if (!skip)
+                  tma_load(dst + h * 16384 + g * a.box * 128, maps + kv, h * 64, y, w.kvh, bar);
+            }
+          }
+          if (ragged) {
+            const int g = __ffs(ragged) - 1;      // the last box only
+            const int y = __shfl_sync(~0u, row, g), n_rows = __shfl_sync(~0u, rows, g);
+            for (int r = 0; r < a.box; ++r)
+              if (elect())
+                for (int h = 0; h < L::kHalves; ++h)
+                  tma_load(dst + h * 16384 + (g * a.box + r) * 128, maps + 2 + kv, h * 64,
+                           r < n_rows ? y + r : outside, w.kvh, bar);
+          }
+          __syncwarp();
+          ++item;
+        }
+      }
+    }
+  }
+}
+
+// The query rows of a work tile, once the last scores of the one before have been
+// computed: by TMA (a box is per_tile tokens by the group's heads by 64 elements,
+// which is the order of the rows) or by two warps that gather.
+template <typename T, int HD, bool kTma>
+__device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t* base, Control* c,
+                           int items) {
+  using L = Layout<HD>;
+  const Params& p = a.p;
+  constexpr int kChunks = HD / 8, kRows = kQLoaders / kChunks;
+  const int t = threadIdx.x & (kQLoaders - 1);
+  const int chunk = t % kChunks, r0 = t / kChunks;
+  const uint32_t q = smem_u32(base + L::kQ), bar = smem_u32(&c->q_full);
+  uint32_t n = 0;
+  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+    Work w;
+    int tile;
+    if (!segment(a, it, w, tile)) continue;
+    for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
+      locate(a, w, tile);
+      if (w.j0 >= w.j1) continue;
+      if (n > 0 && !warp_wait(smem_u32(&c->q_free), (n - 1) & 1, &c->quit)) break;
+      ++n;
+      const int tiles = row_tiles_of(a, w);
+      if (kTma) {
+        if (elect()) {
+          mbar_expect(bar, tiles * L::kHalves * a.per_tile * p.group * 128);
+          for (int s = 0; s < tiles; ++s)
+            for (int h = 0; h < L::kHalves; ++h)
+              tma_load4(q + s * L::kTileBytes + h * 16384, map, h * 64, 0, w.kvh,
+                        w.tok0 + w.first + s * a.per_tile, bar);
+        }
+        __syncwarp();
+      } else {
+        const uint8_t* qb = static_cast<const uint8_t*>(p.q) + chunk * 16;
+#pragma unroll 4
+        for (int r = r0; r < tiles * kTile; r += kRows) {
+          const int tok = p.group_div.div(r % kTile), g = r % kTile - tok * p.group;
+          const int at = w.first + r / kTile * a.per_tile + tok;
+          const bool ok = tok < a.per_tile && at < w.ntok;
+          const uint8_t* src = qb + ((w.tok0 + at) * p.q_token +
+                                     (int64_t)(w.kvh * p.group + g) * p.q_head) * 2;
+          cp_async16(q + (r / kTile) * L::kTileBytes + (chunk / 8) * 16384 + (r % kTile) * 128 +
+                         (((chunk & 7) ^ (r & 7)) << 4),
+                     ok ? src : qb, ok);
+        }
+        cp_commit();
+        cp_wait<0>();
+        fence_proxy_async();
+        mbar_arrive(bar);
+      }
+    }
+  }
+  // a load that nothing waited for (the others gave up) ends before the CTA does
+  if (kTma && c->quit && n > 0) {
+    const long long t0 = clock64();
+    while (!mbar_try(bar, (n - 1) & 1) && clock64() - t0 < kWaitCycles) {
+    }
+  }
+}
+
+template <typename T, int HD>
+__device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int items,
+                           uint32_t tmem_lane) {
+  using L = Layout<HD>;
+  constexpr uint32_t kIdS = idesc<T>(kTile, false), kIdO = idesc<T>(HD, true);
+  constexpr uint32_t kStep = L::kTileBytes >> 4;       // of a descriptor, per stage or row tile
+  const uint32_t leader = elect() ? 1u : 0u;
+  const uint32_t tmem = __shfl_sync(~0u, tmem_lane, 0);   // uniform
+  const uint32_t q_lo = desc_lo(smem_u32(base + L::kQ), 16);
+  const uint32_t k_lo = desc_lo(smem_u32(base + L::kRing), 16);
+  const uint32_t v_lo = desc_lo(smem_u32(base + L::kRing), 16384);
+  const uint32_t full0 = smem_u32(&c->full[0]), empty0 = smem_u32(&c->empty[0]);
+  const uint32_t s_full0 = smem_u32(&c->s_full[0]), p_ready0 = smem_u32(&c->p_ready[0]);
+  const uint32_t o_done0 = smem_u32(&c->o_done[0]);
+  uint32_t np = 0, nq = 0;     // phase bits: of p_ready (bit s), of q_full
+
+  // K and V tiles alternate in the ring: a cursor on the next one, in the order of arrival
+  struct Cursor {
+    uint32_t stage = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+      if (++stage == L::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  } cur;
+  auto full = [&](const Cursor& x) { return warp_wait(full0 + 8 * x.stage, x.phase, &c->quit); };
+  auto release = [&](const Cursor& x) { tc_commit(leader, empty0 + 8 * x.stage); };
+  auto p_ready = [&](int s) {
+    const bool ok = warp_wait(p_ready0 + 8 * s, np >> s & 1, &c->quit);
+    np ^= 1u << s;
+    return ok;
+  };
+  auto scores = [&](int s, int q, const Cursor& x) {      // S_s = Q_q K^T
+    const uint32_t ql = q_lo + q * kStep, kl = k_lo + x.stage * kStep, d = tmem + s * kTile;
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk) {
+      const uint32_t off = ((kk / 4) * 16384 + (kk % 4) * 32) >> 4;
+      mma_ss(leader, d, desc(ql + off), desc(kl + off), kIdS, kk > 0);
+    }
+    tc_commit(leader, s_full0 + 8 * s);
+  };
+  auto product = [&](int s, const Cursor& x, bool first) {   // O_s (+)= P_s V
+    const uint32_t vl = v_lo + x.stage * kStep;
+    const uint32_t d = tmem + 2 * kTile + s * HD, pa = tmem + s * kTile;
+#pragma unroll
+    for (int kk = 0; kk < kTile / 16; ++kk)
+      mma_ts(leader, d, pa + kk * 8, desc(vl + kk * (2048 >> 4)), kIdO, !first || kk > 0);
+  };
+
+  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+    Work w;
+    int tile;
+    if (!segment(a, it, w, tile)) continue;
+    for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
       const int nt = w.j1 - w.j0;
       if (nt <= 0) continue;
+      if (!warp_wait(smem_u32(&c->q_full), nq, &c->quit)) return;
+      nq ^= 1;
       if (a.twin) {
+        Cursor v[2];        // V tile of each stream's last scores
         for (int i = 0; i < nt + 2; ++i) {
           const int s = i & 1;
           if (i >= 2) {       // the product of step i - 2, the same stream
-            const uint32_t v = item + 2 * (i - 2) + 1;
-            if (!p_ready(s) || !full(v)) return;
+            const Cursor x = s ? v[1] : v[0];
+            if (!p_ready(s) || !full(x)) return;
             tc_fence_after();
-            product(s, v, i < 4);
-            release(v);
-            if (i >= nt) tc_commit(smem_u32(&c->o_done[s]));
+            product(s, x, i < 4);
+            release(x);
+            if (i >= nt) tc_commit(leader, o_done0 + 8 * s);
           }
           if (i < nt) {
-            const uint32_t k = item + 2 * i;
-            if (!full(k)) return;
+            if (!full(cur)) return;
             tc_fence_after();
-            scores(s, 0, k);
-            release(k);
+            scores(s, 0, cur);
+            release(cur);
+            cur.next();
+            if (s) v[1] = cur;
+            else v[0] = cur;
+            cur.next();
           }
-          if (i == nt - 1) tc_commit(smem_u32(&c->q_free));
+          if (i == nt - 1) tc_commit(leader, smem_u32(&c->q_free));
         }
       } else {
-        const int streams = w.nrows - w.row0 > kTile ? 2 : 1;
+        const int streams = row_tiles_of(a, w);
+        Cursor v;           // V tile of key tile j - 1
         for (int j = 0; j <= nt; ++j) {
-          const uint32_t k = item + 2 * j, v = k - 1;      // v: of key tile j - 1
-          for (int s = 0; s < streams; ++s) {
+          if (j > 0 && !full(v)) return;
+          if (j < nt && !full(cur)) return;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (s >= streams) break;
             if (j > 0) {
-              if (!p_ready(s) || !full(v)) return;
+              if (!p_ready(s)) return;
               tc_fence_after();
               product(s, v, j == 1);
-              if (j == nt) tc_commit(smem_u32(&c->o_done[s]));
-            }
-            if (j < nt) {
-              if (!full(k)) return;
+              if (j == nt) tc_commit(leader, o_done0 + 8 * s);
+            } else {
               tc_fence_after();
-              scores(s, s, k);
             }
+            if (j < nt) scores(s, s, cur);
           }
           if (j > 0) release(v);
-          if (j < nt) release(k);
-          if (j == nt - 1) tc_commit(smem_u32(&c->q_free));
+          if (j < nt) {
+            release(cur);
+            cur.next();
+            v = cur;
+            cur.next();
+          }
+          if (j == nt - 1) tc_commit(leader, smem_u32(&c->q_free));
         }
       }
-      item += 2 * nt;
     }
   }
 }
@@ -570,6 +824,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;       // this warp's TMEM lanes
   const uint32_t ts = tmem + lanes + s * kTile, to = tmem + lanes + 2 * kTile + s * HD;
   const float scale2 = p.scale2;
+  const int row_tok = p.group_div.div(r), row_head = r - row_tok * p.group;
   uint32_t n_s = 0, n_o = 0;          // s_full and o_done phases waited for
   uint32_t tiles = 0;                 // key tiles of the work tiles before
 
@@ -577,23 +832,22 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
     Work w;
     int tile;
     if (!segment(a, it, w, tile)) continue;
-    for (; tile * rows_of_work(a) < w.nrows; tile += a.row_tiles) {
+    for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
-      const int row = w.row0 + (a.twin ? 0 : s * kTile) + r;
       const uint32_t tile0 = tiles;
       tiles += max(w.j1 - w.j0, 0);
-      if (!a.twin && s == 1 && w.nrows - w.row0 <= kTile) continue;
-      const bool live = row < w.nrows;
-      const int tok = live ? p.group_div.div(row) : 0;
-      const int t = w.tok0 + tok;
-      const int head = w.kvh * p.group + (live ? row - tok * p.group : 0);
+      if (!a.twin && s >= row_tiles_of(a, w)) continue;
+      const int tok = w.first + (a.twin ? 0 : s * a.per_tile) + row_tok;
+      const bool live = row_tok < a.per_tile && tok < w.ntok;
+      const int t = w.tok0 + (live ? tok : 0);
+      const int head = w.kvh * p.group + row_head;
       int pos = -1;
       if (live) pos = a.mode == kPrefix ? position_of(p, sequence_of(p, t), t)
                                         : w.ctx - w.ntok + tok;
       // virtual key v is seen iff v <= vmax and (v >= vmin or v < sinks)
       const int shift = w.lo - w.ns;
       const int vmax = pos < 0 ? -1 : min(pos - shift, w.n - 1);
-      const int vmin = p.window > 0 ? pos - p.window + 1 - shift : -1;
+      const int vmin = max(p.window > 0 ? pos - p.window + 1 : 0, p.key_start) - shift;
 
       float m = -INFINITY, l = 0.0f;
       int done = 0;
@@ -605,17 +859,21 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
         tmem_ld64(ts, raw);
         tmem_ld64(ts + 64, raw + 64);
         const int v0 = j * kTile;
-        const uint4 bad = *reinterpret_cast<const uint4*>(c->invalid[(tile0 + (j - w.j0)) % kInvalidRing]);
+        const uint4 bad = *reinterpret_cast<const uint4*>(
+            c->invalid[(tile0 + (j - w.j0)) % kInvalidRing]);
         const bool whole = v0 + kTile - 1 <= vmax && (v0 >= vmin || v0 + kTile <= p.sinks) &&
                            (bad.x | bad.y | bad.z | bad.w) == 0;
         if (!__all_sync(~0u, whole)) {
+          // the row's visible keys of the tile as 128 bits
           const uint32_t words[4] = {bad.x, bad.y, bad.z, bad.w};
 #pragma unroll
-          for (int i = 0; i < kTile; ++i) {
-            const int v = v0 + i;
-            const bool see = v <= vmax && (v >= vmin || v < p.sinks) &&
-                             !(words[i / 32] >> (i % 32) & 1u);
-            if (!see) raw[i] = 0xFF800000u;
+          for (int i = 0; i < 4; ++i) {
+            const int at = v0 + 32 * i;
+            const uint32_t see = below(vmax + 1 - at) & (~below(vmin - at) | below(p.sinks - at)) &
+                                 ~words[i];
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(see & (1u << e))) raw[32 * i + e] = 0xFF800000u;
           }
         }
         float mx[4];
@@ -672,7 +930,6 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
         ++n_o;
         tc_fence_after();
         inv = l == 0.0f ? 0.0f : (p.slots ? 1.0f : 1.0f / l);
-        check = l * 0.0f;
       }
 #pragma unroll
       for (int h = 0; h < HD; h += 64) {
@@ -692,27 +949,24 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
           o[i] = __float_as_uint(v);
         }
         if (live && p.slots) {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + at * HD + h);
 #pragma unroll
-          for (int i = 0; i < 64; i += 4)
-            dst[i / 4] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
-                                     __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+          for (int i = 0; i < 64; i += 8) store32(p.part_o + at * HD + h + i, o + i, true);
         } else if (live) {
-          uint4* dst = reinterpret_cast<uint4*>(out + h);
 #pragma unroll
-          for (int i = 0; i < 64; i += 8) {
-            uint32_t x[4];
+          for (int i = 0; i < 64; i += 16) {
+            uint32_t x[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 8; ++e)
               x[e] = pack2<T>(__uint_as_float(o[i + 2 * e]), __uint_as_float(o[i + 2 * e + 1]));
-            dst[i / 8] = make_uint4(x[0], x[1], x[2], x[3]);
+            store32(out + h + i, x, a.wide_out);
           }
         }
       }
       if (done > 0) tc_fence_before();       // O has been read before the next P arrives
       if (live && p.slots) p.part_ml[at] = make_float2(m, l);
 
-      uint32_t again = __ballot_sync(~0u, live && !(check == 0.0f));
+      // a sum that is not finite is the row's own: only keys that it sees enter it
+      uint32_t again = __ballot_sync(~0u, live && l - l == 0.0f && !(check == 0.0f));
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
@@ -735,10 +989,11 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
   }
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1)
-attention_tile_kernel(const __grid_constant__ TileParams a) {
+template <typename T, int HD, bool kTma>
+__global__ void __launch_bounds__(Warps<kTma>::kThreads, 1)
+attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constant__ Maps maps) {
   using L = Layout<HD>;
+  using W = Warps<kTma>;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* base = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   Control* c = reinterpret_cast<Control*>(base + L::kControl);
@@ -747,7 +1002,7 @@ attention_tile_kernel(const __grid_constant__ TileParams a) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; ++i) {
-      mbar_init(smem_u32(&c->full[i]), kLoaders);
+      mbar_init(smem_u32(&c->full[i]), kTma ? 1 : kLoaders);
       mbar_init(smem_u32(&c->empty[i]), 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -755,11 +1010,12 @@ attention_tile_kernel(const __grid_constant__ TileParams a) {
       mbar_init(smem_u32(&c->p_ready[s]), kTile);
       mbar_init(smem_u32(&c->o_done[s]), 1);
     }
+    mbar_init(smem_u32(&c->q_full), kTma ? 1 : kQLoaders);
     mbar_init(smem_u32(&c->q_free), 1);
     c->quit = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == W::kIssue) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                      smem_u32(&c->tmem))
                  : "memory");
@@ -770,14 +1026,19 @@ attention_tile_kernel(const __grid_constant__ TileParams a) {
   tc_fence_after();
   const uint32_t tmem = c->tmem;
 
-  // 512 threads at 128 registers: 256 x 192 + 256 x 64 is the same total
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(W::kSoftmaxRegs));
     softmax_role<T, HD>(a, c, items, tmem, warp >> 2);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp < 12) load_role<T, HD>(a, base, c, items);
-    else if (warp == 12 && (threadIdx.x & 31) == 0) issue_role<T, HD>(a, base, c, items, tmem);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::kOtherRegs));
+    if (warp < W::kIssue) {
+      if (kTma) tma_role<T, HD>(a, maps.map, base, c, items);
+      else gather_role<T, HD>(a, base, c, items);
+    } else if (warp == W::kIssue) {
+      issue_role<T, HD>(a, base, c, items, tmem);
+    } else if (warp < W::kQuery + (kTma ? 1 : 2)) {
+      query_role<T, HD, kTma>(a, &maps.q, base, c, items);
+    }
   }
   // every product issued has finished (the softmax warps waited for the last) unless a
   // wait ran out: then give what is in flight the time to end before TMEM goes
@@ -787,44 +1048,114 @@ attention_tile_kernel(const __grid_constant__ TileParams a) {
   __syncthreads();
   tc_fence_after();
   if (c->quit) {
-    if (warp == 12 && (threadIdx.x & 31) == 0) {
+    if (warp == W::kIssue && (threadIdx.x & 31) == 0) {
       mbar_init(smem_u32(&c->slots[0][0]), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      tc_commit(smem_u32(&c->slots[0][0]));
+      tc_commit(1u, smem_u32(&c->slots[0][0]));
       const long long t0 = clock64();
       while (!mbar_try(smem_u32(&c->slots[0][0]), 0) && clock64() - t0 < kWaitCycles) {
       }
     }
     __syncthreads();
   }
-  if (warp == 12)
+  if (warp == W::kIssue)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <typename T, int HD>
-int launch(const TileParams& a, cudaStream_t s) {
-  auto kernel = attention_tile_kernel<T, HD>;
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  return fn;
+}
+
+// K and V as [kv_heads][slots][head], in boxes of 64 elements by `box` rows and by one.
+bool encode(Maps& maps, const Params& p, int dtype, int box) {
+  EncodeFn enc = encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)p.hd, (cuuint64_t)p.cache_rows,
+                              (cuuint64_t)p.kv_heads};
+  const cuuint64_t strides[2] = {(cuuint64_t)p.slot_stride * 2,
+                                 (cuuint64_t)(p.kv_heads > 1 ? p.head_stride : 8) * 2};
+  const cuuint32_t unit[3] = {1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    const cuuint32_t size[3] = {64, i < 2 ? (cuuint32_t)box : 1u, 1};
+    if (enc(&maps.map[i],
+            dtype == IE_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+            3, const_cast<void*>(i & 1 ? p.v : p.k), dims, strides, size, unit,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  }
+  // the query rows as [tokens][kv_heads][group][head]
+  const cuuint64_t q_dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.group, (cuuint64_t)p.kv_heads,
+                                (cuuint64_t)p.tokens};
+  const cuuint64_t head = (cuuint64_t)(p.heads > 1 ? p.q_head : 8) * 2;
+  const cuuint64_t q_strides[3] = {head, head * p.group,
+                                   (cuuint64_t)(p.tokens > 1 ? p.q_token : 8) * 2};
+  const cuuint32_t q_size[4] = {64, (cuuint32_t)p.group, 1, (cuuint32_t)(kTile / p.group)};
+  const cuuint32_t q_unit[4] = {1, 1, 1, 1};
+  return enc(&maps.q,
+             dtype == IE_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+             4, const_cast<void*>(p.q), q_dims, q_strides, q_size, q_unit,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD, bool kTma>
+int launch(const TileParams& a, const Maps& maps, cudaStream_t s) {
+  auto kernel = attention_tile_kernel<T, HD, kTma>;
   IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    Layout<HD>::kBytes));
   const int64_t items = (int64_t)a.row_tiles * a.parts * a.segs * a.p.kv_heads;
-  kernel<<<(unsigned)(items < kSms ? items : kSms), kThreads, Layout<HD>::kBytes, s>>>(a);
+  kernel<<<(unsigned)(items < kSms ? items : kSms), Warps<kTma>::kThreads, Layout<HD>::kBytes,
+           s>>>(a, maps);
   return launch_status("attention_tile_kernel");
+}
+template <typename T>
+int launch(TileParams& a, int dtype, cudaStream_t s) {
+  const Params& p = a.p;
+  Maps maps;
+  // TMA wants boxes of at least 8 rows (a swizzle period) within a page; smaller powers of
+  // two and rows that a tensor map cannot name (a stride of 0) are gathered
+  const int low = (int)(p.block.d & -p.block.d);
+  a.box = low >= kMaxBox ? kMaxBox : low;
+  if (a.box < 8 || p.pages == 0 || p.slot_stride <= 0 || (p.kv_heads > 1 && p.head_stride <= 0) ||
+      (p.tokens > 1 && p.q_token <= 0) || (p.heads > 1 && p.q_head <= 0) ||
+      !encode(maps, p, dtype, a.box))
+    a.box = 0;
+  if (a.box) return p.hd == 64 ? launch<T, 64, true>(a, maps, s) : launch<T, 128, true>(a, maps, s);
+  return p.hd == 64 ? launch<T, 64, false>(a, maps, s) : launch<T, 128, false>(a, maps, s);
 }
 
 }  // namespace
 
 int launch_tiles(const Params& p, int dtype, bool prefix, bool twin, int row_tiles, int parts,
                  cudaStream_t s) {
-  TileParams a;
+  TileParams a{};
   a.p = p;
   a.mode = prefix ? kPrefix : kPrefill;
   a.twin = twin;
+  a.per_tile = kTile / p.group;
   a.row_tiles = row_tiles;
   a.segs = prefix ? 1 : p.seqs;
   a.parts = parts;
-  if (dtype == IE_DT_BF16)
-    return p.hd == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
-  return p.hd == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+  a.wide_out = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_token * 2) % 32 == 0;
+  return dtype == IE_DT_BF16 ? launch<__nv_bfloat16>(a, dtype, s) : launch<__half>(a, dtype, s);
 }
 
 uint32_t attention_status(bool clear) {
