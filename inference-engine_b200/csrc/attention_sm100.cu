@@ -289,6 +289,29 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// ---- exponentials -----------------------------------------------------------------
+// Two f32 in a 64-bit register: one instruction does both.
+__device__ __forceinline__ uint64_t f32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  return f32x2(__float_as_uint(lo), __float_as_uint(hi));
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // ---- shared memory -------------------------------------------------------------
 template <int HD>
 struct Layout {
@@ -301,7 +324,7 @@ struct Layout {
   static constexpr int kBytes = kControl + 2048 + 1024;   // + alignment of the base
 };
 struct Control {
-  uint64_t full[8], empty[8], s_full[2], p_ready[2], o_done[2], q_full, q_free;
+  uint64_t full[8], empty[8], s_full[2], p_ready[2][2], o_done[2], q_full, q_free;
   int slots[2][kTile];                     // cache rows of a key tile
   alignas(16) uint32_t invalid[kInvalidRing][4];   // keys of a tile whose page is not there
   uint32_t tmem;
@@ -712,7 +735,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int i
   const uint32_t k_lo = desc_lo(smem_u32(base + L::kRing), 16);
   const uint32_t v_lo = desc_lo(smem_u32(base + L::kRing), 16384);
   const uint32_t full0 = smem_u32(&c->full[0]), empty0 = smem_u32(&c->empty[0]);
-  const uint32_t s_full0 = smem_u32(&c->s_full[0]), p_ready0 = smem_u32(&c->p_ready[0]);
+  const uint32_t s_full0 = smem_u32(&c->s_full[0]), p_ready0 = smem_u32(&c->p_ready[0][0]);
   const uint32_t o_done0 = smem_u32(&c->o_done[0]);
   uint32_t np = 0, nq = 0;     // phase bits: of p_ready (bit s), of q_full
 
@@ -728,10 +751,8 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int i
   } cur;
   auto full = [&](const Cursor& x) { return warp_wait(full0 + 8 * x.stage, x.phase, &c->quit); };
   auto release = [&](const Cursor& x) { tc_commit(leader, empty0 + 8 * x.stage); };
-  auto p_ready = [&](int s) {
-    const bool ok = warp_wait(p_ready0 + 8 * s, np >> s & 1, &c->quit);
-    np ^= 1u << s;
-    return ok;
+  auto p_ready = [&](int s, int half) {
+    return warp_wait(p_ready0 + 16 * s + 8 * half, np >> s & 1, &c->quit);
   };
   auto scores = [&](int s, int q, const Cursor& x) {      // S_s = Q_q K^T
     const uint32_t ql = q_lo + q * kStep, kl = k_lo + x.stage * kStep, d = tmem + s * kTile;
@@ -745,9 +766,17 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int i
   auto product = [&](int s, const Cursor& x, bool first) {   // O_s (+)= P_s V
     const uint32_t vl = v_lo + x.stage * kStep;
     const uint32_t d = tmem + 2 * kTile + s * HD, pa = tmem + s * kTile;
+    // the first half of the weights arrives while the exponentials of the second run
 #pragma unroll
-    for (int kk = 0; kk < kTile / 16; ++kk)
-      mma_ts(leader, d, pa + kk * 8, desc(vl + kk * (2048 >> 4)), kIdO, !first || kk > 0);
+    for (int half = 0; half < 2; ++half) {
+      if (!p_ready(s, half)) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+        mma_ts(leader, d, pa + kk * 8, desc(vl + kk * (2048 >> 4)), kIdO, !first || kk > 0);
+    }
+    np ^= 1u << s;
+    return true;
   };
 
   for (int it = blockIdx.x; it < items; it += gridDim.x) {
@@ -766,9 +795,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int i
           const int s = i & 1;
           if (i >= 2) {       // the product of step i - 2, the same stream
             const Cursor x = s ? v[1] : v[0];
-            if (!p_ready(s) || !full(x)) return;
-            tc_fence_after();
-            product(s, x, i < 4);
+            if (!full(x) || !product(s, x, i < 4)) return;
             release(x);
             if (i >= nt) tc_commit(leader, o_done0 + 8 * s);
           }
@@ -794,9 +821,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int i
           for (int s = 0; s < 2; ++s) {
             if (s >= streams) break;
             if (j > 0) {
-              if (!p_ready(s)) return;
-              tc_fence_after();
-              product(s, v, j == 1);
+              if (!product(s, v, j == 1)) return;
               if (j == nt) tc_commit(leader, o_done0 + 8 * s);
             } else {
               tc_fence_after();
@@ -824,6 +849,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;       // this warp's TMEM lanes
   const uint32_t ts = tmem + lanes + s * kTile, to = tmem + lanes + 2 * kTile + s * HD;
   const float scale2 = p.scale2;
+  const uint64_t scale22 = f32x2(scale2, scale2);
   const int row_tok = p.group_div.div(r), row_head = r - row_tok * p.group;
   uint32_t n_s = 0, n_o = 0;          // s_full and o_done phases waited for
   uint32_t tiles = 0;                 // key tiles of the work tiles before
@@ -864,16 +890,18 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
         const bool whole = v0 + kTile - 1 <= vmax && (v0 >= vmin || v0 + kTile <= p.sinks) &&
                            (bad.x | bad.y | bad.z | bad.w) == 0;
         if (!__all_sync(~0u, whole)) {
-          // the row's visible keys of the tile as 128 bits
           const uint32_t words[4] = {bad.x, bad.y, bad.z, bad.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
+            // the row's visible keys of these 32 as bits
             const int at = v0 + 32 * i;
             const uint32_t see = below(vmax + 1 - at) & (~below(vmin - at) | below(p.sinks - at)) &
                                  ~words[i];
+            if (!__all_sync(~0u, see == ~0u)) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(see & (1u << e))) raw[32 * i + e] = 0xFF800000u;
+              for (int e = 0; e < 32; ++e)
+                if (!(see & (1u << e))) raw[32 * i + e] = 0xFF800000u;
+            }
           }
         }
         float mx[4];
@@ -899,24 +927,33 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t ref2 = f32x2(-ref, -ref);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i0 = 0; i0 < kTile; i0 += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float w0 = ex2(fmaf(__uint_as_float(raw[i0 + i]), scale2, -ref));
-            const float w1 = ex2(fmaf(__uint_as_float(raw[i0 + i + 1]), scale2, -ref));
-            sum[i & 2] += w0;
-            sum[(i & 2) + 1] += w1;
+            const uint64_t x = fma2(f32x2(raw[i0 + i], raw[i0 + i + 1]), scale22, ref2);
+            float w0, w1;
+            unpack2(x, w0, w1);
+            w0 = ex2(w0);
+            w1 = ex2(w1);
+            sum[i / 2 & 1] = add2(sum[i / 2 & 1], f32x2(w0, w1));
             pk[i / 2] = pack2<T>(w0, w1);
           }
           tmem_st16(ts + i0 / 2, pk);
+          if (i0 % 64 == 32) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&c->p_ready[s][i0 / 64]));
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(smem_u32(&c->p_ready[s]));
+        {
+          float s0, s1;
+          unpack2(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
+        }
         ++done;
       }
 
@@ -1007,7 +1044,8 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(smem_u32(&c->s_full[s]), 1);
-      mbar_init(smem_u32(&c->p_ready[s]), kTile);
+      mbar_init(smem_u32(&c->p_ready[s][0]), kTile);
+      mbar_init(smem_u32(&c->p_ready[s][1]), kTile);
       mbar_init(smem_u32(&c->o_done[s]), 1);
     }
     mbar_init(smem_u32(&c->q_full), kTma ? 1 : kQLoaders);
