@@ -65,9 +65,12 @@ __device__ uint32_t g_attention_status = 0;
 enum Mode { kPrefill = 0, kPrefix = 1 };
 
 // Warps: 0-7 softmax, then the loaders of K and V (one warp with TMA, four that
-// gather), the issuing warp and two that load the query rows.
+// gather), the issuing warp, one or two that load the query rows and the one that
+// fetches the next work item.
 template <bool kTma> struct Warps {
-  static constexpr int kIssue = kTma ? 9 : 12, kQuery = kIssue + 1;
+  static constexpr int kIssue = kTma ? 9 : 12, kQuery = kIssue + 1, kNext = kTma ? 11 : 15;
+  // warps that read the work item: all but the one that fetches it
+  static constexpr int kReaders = kTma ? 11 : 15;
   static constexpr int kThreads = kTma ? 384 : 512;
   // registers of the softmax warps and of the others: together the launch's
   // (384 x 168: 256 x 208 + 128 x 88; 512 x 128: 256 x 192 + 256 x 64)
@@ -325,12 +328,77 @@ struct Layout {
 };
 struct Control {
   uint64_t full[8], empty[8], s_full[2], p_ready[2][2], o_done[2], q_full, q_free;
+  uint64_t next_full, next_empty;          // the next work item
+  alignas(16) uint32_t next[4];
   int slots[2][kTile];                     // cache rows of a key tile
   alignas(16) uint32_t invalid[kInvalidRing][4];   // keys of a tile whose page is not there
   uint32_t tmem;
   int quit;
 };
 static_assert(sizeof(Control) <= 2048, "control block");
+
+// ---- work items --------------------------------------------------------------------
+// The grid has a CTA for every work item.  A resident CTA takes over, one at a time,
+// CTAs that have not been launched yet (cluster launch control), so items of uneven
+// length spread over the SMs as they come free, and the loads of the next item
+// run under the end of the last.
+__device__ __forceinline__ void try_take(uint32_t answer, uint32_t bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+      "[%0], [%1];" ::"r"(answer),
+      "r"(bar)
+      : "memory");
+}
+// The item that was taken, or -1.
+__device__ __forceinline__ int taken(uint32_t answer) {
+  uint32_t x, ok;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+      : "=r"(x), "=r"(ok)
+      : "r"(answer)
+      : "memory");
+  return ok ? (int)x : -1;
+}
+// A reader's way through the items: the CTA's own, then what it takes over.
+struct Items {
+  uint32_t phase = 0;
+  int item;
+  __device__ __forceinline__ explicit Items(int first) : item(first) {}
+  // -1: no more (or another role gave up)
+  __device__ __forceinline__ void next(Control* c) {
+    if (!warp_wait(smem_u32(&c->next_full), phase, &c->quit)) {
+      item = -1;
+      return;
+    }
+    phase ^= 1;
+    item = taken(smem_u32(c->next));
+    fence_proxy_async();
+    __syncwarp();
+    if (elect()) mbar_arrive(smem_u32(&c->next_empty));
+  }
+};
+// The warp that takes them over; it never asks again after a refusal.
+__device__ __forceinline__ void next_role(Control* c) {
+  const uint32_t full = smem_u32(&c->next_full);
+  for (uint32_t n = 0;; ++n) {
+    if (n > 0 && !warp_wait(smem_u32(&c->next_empty), (n - 1) & 1, &c->quit)) return;
+    if (elect()) {
+      mbar_expect(full, 16);
+      try_take(smem_u32(c->next), full);
+    }
+    __syncwarp();
+    const long long t0 = clock64();      // what was asked arrives before the CTA ends
+    while (!mbar_try(full, n & 1) && clock64() - t0 < kWaitCycles) {
+    }
+    __syncwarp();
+    if (taken(smem_u32(c->next)) < 0) return;
+  }
+}
 
 // ---- work ------------------------------------------------------------------------
 // One work tile: the tokens from `first` on of a segment (two row tiles of
@@ -464,7 +532,7 @@ __device__ __forceinline__ uint32_t below(int n) {
 
 // ---- roles ---------------------------------------------------------------------------
 template <typename T, int HD>
-__device__ void gather_role(const TileParams& a, uint8_t* base, Control* c, int items) {
+__device__ void gather_role(const TileParams& a, uint8_t* base, Control* c) {
   using L = Layout<HD>;
   const Params& p = a.p;
   constexpr int kChunks = HD / 8;                  // 16-byte chunks of a row
@@ -522,10 +590,16 @@ __device__ void gather_role(const TileParams& a, uint8_t* base, Control* c, int 
     }
   };
 
-  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+  auto next_item = [&](Items& it) {
+    flush();                               // the wait below is for those who use the loads
+    it.next(c);
+    return !any_failed(it.item < 0 || failed);       // all of the loaders go on, or none
+  };
+  Items it(blockIdx.x);
+  do {
     Work w;
     int tile;
-    if (!segment(a, it, w, tile)) continue;
+    if (!segment(a, it.item, w, tile)) continue;
     const int32_t* table = p.tables + (a.mode == kPrefix ? 0 : (int64_t)w.seg * p.table_stride);
     const uint8_t* kb = static_cast<const uint8_t*>(p.k) + (int64_t)w.kvh * p.head_stride * 2 +
                         chunk * 16;
@@ -563,7 +637,7 @@ __device__ void gather_role(const TileParams& a, uint8_t* base, Control* c, int 
         }
       }
     }
-  }
+  } while (next_item(it));
   flush();
 }
 
@@ -572,8 +646,7 @@ __device__ void gather_role(const TileParams& a, uint8_t* base, Control* c, int 
 // tile, one lane issues them all.  A box whose page is not there, and rows past the
 // last key, are read outside the tensor: zeros.
 template <typename T, int HD>
-__device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* base, Control* c,
-                         int items) {
+__device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* base, Control* c) {
   using L = Layout<HD>;
   const Params& p = a.p;
   const int lane = threadIdx.x & 31;
@@ -583,10 +656,10 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
   const int outside = p.cache_rows;
   uint32_t item = 0;
 
-  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+  for (Items it(blockIdx.x); it.item >= 0; it.next(c)) {
     Work w;
     int tile;
-    if (!segment(a, it, w, tile)) continue;
+    if (!segment(a, it.item, w, tile)) continue;
     const int32_t* table = p.tables + (a.mode == kPrefix ? 0 : (int64_t)w.seg * p.table_stride);
     for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
@@ -667,8 +740,7 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
 // computed: by TMA (a box is per_tile tokens by the group's heads by 64 elements,
 // which is the order of the rows) or by two warps that gather.
 template <typename T, int HD, bool kTma>
-__device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t* base, Control* c,
-                           int items) {
+__device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t* base, Control* c) {
   using L = Layout<HD>;
   const Params& p = a.p;
   constexpr int kChunks = HD / 8, kRows = kQLoaders / kChunks;
@@ -676,10 +748,10 @@ __device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t*
   const int chunk = t % kChunks, r0 = t / kChunks;
   const uint32_t q = smem_u32(base + L::kQ), bar = smem_u32(&c->q_full);
   uint32_t n = 0;
-  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+  for (Items it(blockIdx.x); it.item >= 0; it.next(c)) {
     Work w;
     int tile;
-    if (!segment(a, it, w, tile)) continue;
+    if (!segment(a, it.item, w, tile)) continue;
     for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
       if (w.j0 >= w.j1) continue;
@@ -724,7 +796,7 @@ __device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t*
 }
 
 template <typename T, int HD>
-__device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int items,
+__device__ void issue_role(const TileParams& a, uint8_t* base, Control* c,
                            uint32_t tmem_lane) {
   using L = Layout<HD>;
   constexpr uint32_t kIdS = idesc<T>(kTile, false), kIdO = idesc<T>(HD, true);
@@ -779,10 +851,10 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int i
     return true;
   };
 
-  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+  for (Items it(blockIdx.x); it.item >= 0; it.next(c)) {
     Work w;
     int tile;
-    if (!segment(a, it, w, tile)) continue;
+    if (!segment(a, it.item, w, tile)) continue;
     for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
       const int nt = w.j1 - w.j0;
@@ -843,7 +915,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c, int i
 }
 
 template <typename T, int HD>
-__device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_t tmem, int s) {
+__device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int s) {
   const Params& p = a.p;
   const int r = threadIdx.x & (kTile - 1), lane = threadIdx.x & 31;
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;       // this warp's TMEM lanes
@@ -854,10 +926,10 @@ __device__ void softmax_role(const TileParams& a, Control* c, int items, uint32_
   uint32_t n_s = 0, n_o = 0;          // s_full and o_done phases waited for
   uint32_t tiles = 0;                 // key tiles of the work tiles before
 
-  for (int it = blockIdx.x; it < items; it += gridDim.x) {
+  for (Items it(blockIdx.x); it.item >= 0; it.next(c)) {
     Work w;
     int tile;
-    if (!segment(a, it, w, tile)) continue;
+    if (!segment(a, it.item, w, tile)) continue;
     for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
       const uint32_t tile0 = tiles;
@@ -1035,7 +1107,6 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
   uint8_t* base = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   Control* c = reinterpret_cast<Control*>(base + L::kControl);
   const int warp = threadIdx.x >> 5;
-  const int items = a.row_tiles * a.parts * a.segs * a.p.kv_heads;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; ++i) {
@@ -1050,6 +1121,8 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
     }
     mbar_init(smem_u32(&c->q_full), kTma ? 1 : kQLoaders);
     mbar_init(smem_u32(&c->q_free), 1);
+    mbar_init(smem_u32(&c->next_full), 1);
+    mbar_init(smem_u32(&c->next_empty), W::kReaders);
     c->quit = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -1066,16 +1139,18 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(W::kSoftmaxRegs));
-    softmax_role<T, HD>(a, c, items, tmem, warp >> 2);
+    softmax_role<T, HD>(a, c, tmem, warp >> 2);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::kOtherRegs));
     if (warp < W::kIssue) {
-      if (kTma) tma_role<T, HD>(a, maps.map, base, c, items);
-      else gather_role<T, HD>(a, base, c, items);
+      if (kTma) tma_role<T, HD>(a, maps.map, base, c);
+      else gather_role<T, HD>(a, base, c);
     } else if (warp == W::kIssue) {
-      issue_role<T, HD>(a, base, c, items, tmem);
+      issue_role<T, HD>(a, base, c, tmem);
     } else if (warp < W::kQuery + (kTma ? 1 : 2)) {
-      query_role<T, HD, kTma>(a, &maps.q, base, c, items);
+      query_role<T, HD, kTma>(a, &maps.q, base, c);
+    } else if (warp == W::kNext) {
+      next_role(c);
     }
   }
   // every product issued has finished (the softmax warps waited for the last) unless a
@@ -1160,7 +1235,7 @@ int launch(const TileParams& a, const Maps& maps, cudaStream_t s) {
   IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    Layout<HD>::kBytes));
   const int64_t items = (int64_t)a.row_tiles * a.parts * a.segs * a.p.kv_heads;
-  kernel<<<(unsigned)(items < kSms ? items : kSms), Warps<kTma>::kThreads, Layout<HD>::kBytes,
+  kernel<<<(unsigned)items, Warps<kTma>::kThreads, Layout<HD>::kBytes,
            s>>>(a, maps);
   return launch_status("attention_tile_kernel");
 }
