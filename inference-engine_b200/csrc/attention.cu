@@ -99,7 +99,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Plan {
   bool simt, decode, prefix;        // which kernels
   int simt_parts;
-  int decode_parts, decode_per;     // one token per sequence, own keys
+  int decode_parts, decode_per, decode_warps;     // one token per sequence, own keys
   bool twin, prefix_twin;           // row tiles: own keys, shared prefix
   int row_tiles, tile_parts, prefix_row_tiles, prefix_parts;
   int slots;                        // 0: a single part, written to out directly
@@ -199,6 +199,8 @@ Plan make_plan(const ie_attention_args& a) {
     plan.decode = true;
     const int64_t units = a.seqs * a.kv_heads * ceil_div(group, 16);
     choose_decode(a, units, own, plan);
+    const int64_t ctas = units * plan.decode_parts;
+    plan.decode_warps = ctas <= kSms ? 8 : 4;
     plan.decode_per = (int)(ceil_div(ceil_div(own, 64), plan.decode_parts) * 64);
   } else {
     const int64_t queries = a.max_query_len > 0 ? std::min(a.max_query_len, a.tokens) : a.tokens;
@@ -247,7 +249,7 @@ int run(const ie_attention_args& a, void* workspace, size_t workspace_bytes, con
     }
     if (plan.decode) {
       p.parts = plan.decode_parts;
-      if (int rc = launch_decode(p, a.dtype, plan.decode_per, s)) return rc;
+      if (int rc = launch_decode(p, a.dtype, plan.decode_per, plan.decode_warps, plan.prefix, s)) return rc;
     } else if (int rc = launch_tiles(p, a.dtype, false, plan.twin, plan.row_tiles,
                                      plan.tile_parts, s)) {
       return rc;

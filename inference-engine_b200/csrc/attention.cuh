@@ -110,6 +110,31 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Programmatic dependent launch: a kernel lets the next one of the stream start when all
+// of its CTAs have said so, and that one waits before it touches what it writes.
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... A, typename... B>
+int launch_pdl(void (*kernel)(A...), int64_t grid, int threads, int smem, cudaStream_t s,
+               bool dependent, const B&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  IE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return IE_OK;
+}
+
 constexpr int kSms = 148;
 constexpr int kMaxDecodeCluster = 8;
 
@@ -117,7 +142,10 @@ constexpr int kMaxDecodeCluster = 8;
 // One token per sequence, 16-bit rows of 64 or 128 elements (attention_decode.cu);
 // part i of a row covers its visible keys [i * per, (i + 1) * per), the last one
 // to the end.  Several parts without slots form clusters (at most 8 parts).
-int launch_decode(const Params& p, int dtype, int per, cudaStream_t s);
+// `after_tiles`: the kernel before on the stream is launch_tiles' of the same call; the
+// two write different slots and run side by side.
+int launch_decode(const Params& p, int dtype, int per, int warps, bool after_tiles,
+                  cudaStream_t s);
 // Rows in tiles on the tensor cores (attention_sm100.cu): every sequence's queries
 // over its own table, or (prefix) all queries over the first table row's keys below
 // key_end.  Part i writes slot slot0 + i, or, twin, slots slot0 + 2 i and 2 i + 1.

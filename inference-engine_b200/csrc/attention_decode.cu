@@ -127,6 +127,9 @@ attention_decode_kernel(const Params p, const int per) {
   const int k1 = part == p.parts - 1 ? keys.n : min(k0 + per, keys.n);
   const int64_t row0 = (int64_t)seq * p.heads + head0;
 
+  // The join may be launched.  What it reads is written by this kernel and the one before
+  // it: this one ends after both.
+  pdl_trigger();
   if (!kCluster && k0 >= k1) {     // nothing of this row lies in this part
     if (p.slots) {
       if (threadIdx.x < rows)
@@ -135,6 +138,7 @@ attention_decode_kernel(const Params p, const int per) {
       T* out = static_cast<T*>(p.out) + seq * p.out_token + (int64_t)head0 * HD;
       for (int i = threadIdx.x; i < rows * HD; i += kWarps * 32) out[i] = from_f32<T>(0.0f);
     }
+    pdl_wait();
     return;
   }
 
@@ -351,44 +355,50 @@ attention_decode_kernel(const Params p, const int per) {
     }
     cluster.sync();      // the others have read this CTA's part
   }
+  pdl_wait();
 }
 
 template <typename T, int HD, int kWarps, bool kCluster>
-int launch(const Params& p, int per, cudaStream_t s) {
+int launch(const Params& p, int per, bool after_tiles, cudaStream_t s) {
   auto kernel = attention_decode_kernel<T, HD, kWarps, kCluster>;
-  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   smem_bytes<HD, kWarps>()));
+  constexpr int kSmem = smem_bytes<HD, kWarps>();
+  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  const int64_t grid = (int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts;
+  if (!kCluster) return launch_pdl(kernel, grid, kWarps * 32, kSmem, s, after_tiles, p, per);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts));
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = smem_bytes<HD, kWarps>();
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
-  if (kCluster) {
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = p.parts;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-  }
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   IE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, per));
   return IE_OK;
 }
 template <typename T, int HD>
-int launch(const Params& p, int per, cudaStream_t s) {
+int launch(const Params& p, int per, int warps, bool after_tiles, cudaStream_t s) {
   const bool cluster = p.parts > 1 && p.slots == 0;
-  const int64_t ctas = (int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts;
-  if (ctas <= kSms)
-    return cluster ? launch<T, HD, 8, true>(p, per, s) : launch<T, HD, 8, false>(p, per, s);
-  return cluster ? launch<T, HD, 4, true>(p, per, s) : launch<T, HD, 4, false>(p, per, s);
+  if (cluster)
+    return warps == 8 ? launch<T, HD, 8, true>(p, per, false, s)
+                      : launch<T, HD, 4, true>(p, per, false, s);
+  if (warps == 8) return launch<T, HD, 8, false>(p, per, after_tiles, s);
+  if (warps == 4) return launch<T, HD, 4, false>(p, per, after_tiles, s);
+  return launch<T, HD, 2, false>(p, per, after_tiles, s);
 }
 
 }  // namespace
 
-int launch_decode(const Params& p, int dtype, int per, cudaStream_t s) {
+int launch_decode(const Params& p, int dtype, int per, int warps, bool after_tiles,
+                  cudaStream_t s) {
   if (dtype == IE_DT_BF16)
-    return p.hd == 64 ? launch<__nv_bfloat16, 64>(p, per, s) : launch<__nv_bfloat16, 128>(p, per, s);
-  return p.hd == 64 ? launch<__half, 64>(p, per, s) : launch<__half, 128>(p, per, s);
+    return p.hd == 64 ? launch<__nv_bfloat16, 64>(p, per, warps, after_tiles, s)
+                      : launch<__nv_bfloat16, 128>(p, per, warps, after_tiles, s);
+  return p.hd == 64 ? launch<__half, 64>(p, per, warps, after_tiles, s)
+                    : launch<__half, 128>(p, per, warps, after_tiles, s);
 }
 
 }  // namespace attn

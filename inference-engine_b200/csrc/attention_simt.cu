@@ -113,30 +113,72 @@ attention_simt_kernel(const Params p) {
   }
 }
 
-// One warp joins the parts of one row: weights 2^(m_i - max m), in slot order.
-template <typename T, int NE>
+// Joins the parts of a row: o = sum o_i 2^(m_i - max m) / sum l_i 2^(m_i - max m), in
+// slot order within each warp.  kSplit warps share a row's slots (few rows: what
+// counts is the latency of the loads, so they are spread and issued eight at a
+// time); its launch and reading overlap the tail of the kernel before it.
+template <typename T, int NE, int kSplit>
 __global__ void __launch_bounds__(128)
 attention_join_kernel(const Params p) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (r >= (int64_t)p.tokens * p.heads) return;
-  const float2* ml = p.part_ml + r * p.slots;
-  float m = -INFINITY;
-  for (int i = lane; i < p.slots; i += 32) m = fmaxf(m, ml[i].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  const float ref = m == -INFINITY ? 0.0f : m;
+  constexpr int kRows = 4 / kSplit;             // rows of a CTA
+  __shared__ float s_o[4][NE * 32];
+  __shared__ float s_l[4];
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kRows + warp / kSplit;
+  const bool live = r < (int64_t)p.tokens * p.heads;
+  const int part = warp % kSplit;
   float l = 0.0f, acc[NE] = {};
-  for (int i = 0; i < p.slots; ++i) {
-    const float2 x = ml[i];
-    if (x.y == 0.0f) continue;
-    const float w = ex2(x.x - ref);
-    l = fmaf(x.y, w, l);
-    const float* o = p.part_o + (r * p.slots + i) * p.hd;
+  if (live) {
+    const float2* ml = p.part_ml + r * p.slots;
+    float m = -INFINITY;
+    for (int i = lane; i < p.slots; i += 32) m = fmaxf(m, ml[i].x);
 #pragma unroll
-    for (int e = 0; e < NE; ++e)
-      if (lane + 32 * e < p.hd) acc[e] = fmaf(o[lane + 32 * e], w, acc[e]);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    for (int i0 = 0; i0 < p.slots; i0 += 32) {
+      // lane i: the weight and the sum of slot i0 + i (0: nothing was seen there)
+      const float2 x = i0 + lane < p.slots ? ml[i0 + lane] : make_float2(-INFINITY, 0.0f);
+      const float w = x.y == 0.0f ? 0.0f : ex2(x.x - ref);
+      const int n = min(32, p.slots - i0);
+      constexpr int kAtOnce = 8;
+      for (int i = part; i < n; i += kSplit * kAtOnce) {
+        float v[kAtOnce][NE], wi[kAtOnce], li[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int q = i + u * kSplit;
+          wi[u] = __shfl_sync(~0u, w, q & 31);
+          li[u] = __shfl_sync(~0u, x.y, q & 31);
+          const bool there = q < n && li[u] != 0.0f;     // otherwise nothing was written
+          if (!there) li[u] = wi[u] = 0.0f;
+          const float* o = p.part_o + (r * p.slots + i0 + q) * p.hd;
+#pragma unroll
+          for (int e = 0; e < NE; ++e)
+            v[u][e] = there && lane + 32 * e < p.hd ? __ldcg(o + lane + 32 * e) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          l = fmaf(li[u], wi[u], l);
+#pragma unroll
+          for (int e = 0; e < NE; ++e) acc[e] = fmaf(v[u][e], wi[u], acc[e]);
+        }
+      }
+    }
   }
+  if (kSplit > 1) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s_o[warp][lane + 32 * e] = acc[e];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int q = 1; q < kSplit; ++q) {
+      l += s_l[warp + q];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) acc[e] += s_o[warp + q][lane + 32 * e];
+    }
+  }
+  if (!live) return;
   const int64_t t = r / p.heads, h = r - t * p.heads;
   T* out = static_cast<T*>(p.out) + t * p.out_token + h * p.hd;
 #pragma unroll
@@ -153,8 +195,9 @@ int simt(const Params& p, cudaStream_t s) {
 template <typename T, int NE>
 int join(const Params& p, cudaStream_t s) {
   const int64_t rows = (int64_t)p.tokens * p.heads;
-  attention_join_kernel<T, NE><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
-  return launch_status("attention_join_kernel");
+  if (rows <= kSms * 8)
+    return launch_pdl(attention_join_kernel<T, NE, 4>, rows, 128, 0, s, true, p);
+  return launch_pdl(attention_join_kernel<T, NE, 1>, (rows + 3) / 4, 128, 0, s, true, p);
 }
 template <typename T>
 int by_size(const Params& p, bool joins, cudaStream_t s) {

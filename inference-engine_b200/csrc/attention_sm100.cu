@@ -687,6 +687,9 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
         const int rows = row < 0 ? 0 : min(w.n - (j * kTile + v_lane), a.box);
         const uint32_t ragged = __ballot_sync(~0u, rows > 0 && rows < a.box);
         const int at = rows > 0 ? row : outside;
+        int y[kTile / 8];                 // every lane: the rows of all boxes
+#pragma unroll
+        for (int g = 0; g < kTile / 8; ++g) y[g] = __shfl_sync(~0u, at, g);
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t st = item % L::kStages, bar = smem_u32(&c->full[st]);
@@ -708,25 +711,24 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
           }
           __syncwarp();
           const uint32_t dst = ring + st * L::kTileBytes;
-#pragma unroll 8
-          for (int g = 0; g < groups; ++g) {
-            const int y = __shfl_sync(~0u, at, g);
-            const int skip = ragged >> g & 1;
-            if (elect()) {
+          if (elect()) {
 #pragma unroll
-              for (int h = 0; h < L::kHalves; ++h)
-                if (!skip)
-                  tma_load(dst + h * 16384 + g * a.box * 128, maps + kv, h * 64, y, w.kvh, bar);
+            for (int g = 0; g < kTile / 8; ++g) {
+              if (g < groups && !(ragged >> g & 1)) {
+#pragma unroll
+                for (int h = 0; h < L::kHalves; ++h)
+                  tma_load(dst + h * 16384 + g * a.box * 128, maps + kv, h * 64, y[g], w.kvh, bar);
+              }
             }
           }
           if (ragged) {
             const int g = __ffs(ragged) - 1;      // the last box only
-            const int y = __shfl_sync(~0u, row, g), n_rows = __shfl_sync(~0u, rows, g);
+            const int y0 = __shfl_sync(~0u, row, g), n_rows = __shfl_sync(~0u, rows, g);
             for (int r = 0; r < a.box; ++r)
               if (elect())
                 for (int h = 0; h < L::kHalves; ++h)
                   tma_load(dst + h * 16384 + (g * a.box + r) * 128, maps + 2 + kv, h * 64,
-                           r < n_rows ? y + r : outside, w.kvh, bar);
+                           r < n_rows ? y0 + r : outside, w.kvh, bar);
           }
           __syncwarp();
           ++item;
@@ -1132,6 +1134,9 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // own keys (decode) or the join may be launched: they wait for this kernel where they
+  // need it
+  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
