@@ -200,7 +200,14 @@ Plan make_plan(const ie_attention_args& a) {
     const int64_t units = a.seqs * a.kv_heads * ceil_div(group, 16);
     choose_decode(a, units, own, plan);
     const int64_t ctas = units * plan.decode_parts;
-    plan.decode_warps = ctas <= kSms ? 8 : 4;
+    // Eight warps an SM, as one CTA or two.  Rows that a window makes equally long also
+    // fill one round of four (64 sequences, window 4096: 151 us against 157; uneven
+    // ones lose: 32 sequences of up to 32768 448 against 356).
+    const bool even = a.window > 0 && a.window + a.sinks < keys;
+    plan.decode_warps = ctas <= kSms ? 8
+                        : even && plan.decode_parts == 1 && ctas > 2 * kSms && ctas <= 4 * kSms
+                            ? 2
+                            : 4;
     plan.decode_per = (int)(ceil_div(ceil_div(own, 64), plan.decode_parts) * 64);
   } else {
     const int64_t queries = a.max_query_len > 0 ? std::min(a.max_query_len, a.tokens) : a.tokens;

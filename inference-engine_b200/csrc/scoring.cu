@@ -9,16 +9,17 @@
 // (e^x = 2^(x log2 e)), and merged by the usual rescaling.
 //
 // The pass is bound by HBM (f32: one exponential per 4 bytes; bf16: near the
-// issue limit too, so a logit costs one max, one FMA, one ex2, one clamp and two
-// accumulations and nothing for the top list).  For the list a thread keeps,
+// exponentials' limit, 16 a cycle and SM: so a logit costs one of those, a clamp, the
+// unpacking and half of a maximum, two FMAs and an addition on packed pairs, and
+// nothing for the top list; the next batch's loads are in flight meanwhile).  For the list a thread keeps,
 // per batch of four 16-byte vectors, only the batch's largest value in shared
-// memory.  After the pass the largest of every four lanes form 128 groups with
-// distinct elements, so the top-th largest group maximum T is a lower bound of
-// the row's top-th element; only batches that reach T are read again (from L2),
-// the few elements at or above T are collected and ranked by counting.
-// Elements are ordered by (value, lower index first) as one 64-bit key, so equal
-// logits - a vocabulary mask's -inf among them - cost no more than distinct
-// ones and the list does not depend on the order of the atomics.
+// memory.  After the pass the largest of every few lanes form groups with distinct
+// elements, so the top-th largest group maximum is a lower bound of the row's
+// top-th element; only batches that reach it are read again (from L2, a warp a
+// batch) and the few elements at or above it are ranked by counting, as 64-bit
+// (value, lower index first) keys.  Where very many equal the bound - a vocabulary
+// mask's -inf, a constant row - those above it are collected and the equal ones
+// taken in index order.  The list does not depend on the order of the atomics.
 //
 // Few rows are split over a thread-block cluster (up to 8 CTAs a row), merged
 // through distributed shared memory: one launch, no workspace.
@@ -31,19 +32,18 @@ namespace score_detail {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;     // four CTAs an SM: one's selection runs under the others' loads
 constexpr int kWarps = kThreads / 32;
 constexpr int kVecs = 4;          // 16-byte vectors of one thread's batch
-constexpr int kGroups = 128;      // four lanes each
 constexpr int kMaxTop = IE_LOGPROBS_MAX_TOP;
-constexpr int kCap = 2048;        // collected candidates
+constexpr int kCap = 1024;        // collected candidates, and batches to look at
 constexpr int kMaxBatches = 16384;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1000.0f;  // 2^kFar == 0: bounds (x - m) where its weight is zero
 
-static_assert(kMaxTop < kGroups, "the threshold is the top-th group maximum");
+static_assert(kMaxTop <= kThreads / 2, "the bound is the top-th of the group maxima");
 
 // (value, lower index first) as an unsigned key; NaN ranks with -inf.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -115,6 +115,70 @@ __device__ __forceinline__ void unpack<__half>(uint4 v, float* x) {
   }
 }
 
+// The largest of a vector's elements and of `m`; NaN only if all are.
+template <typename T>
+struct Max {
+  uint32_t m;      // a pair of T; f32: one
+  __device__ __forceinline__ void start(uint4 v);
+  __device__ __forceinline__ void add(uint4 v);
+  __device__ __forceinline__ float value() const;
+};
+template <>
+__device__ __forceinline__ void Max<float>::start(uint4 v) {
+  m = __float_as_uint(fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                            fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+}
+template <>
+__device__ __forceinline__ void Max<float>::add(uint4 v) {
+  Max<float> o;
+  o.start(v);
+  m = __float_as_uint(fmaxf(__uint_as_float(m), __uint_as_float(o.m)));
+}
+template <>
+__device__ __forceinline__ float Max<float>::value() const { return __uint_as_float(m); }
+template <typename H2>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  const H2 r = __hmax2(*reinterpret_cast<const H2*>(&a), *reinterpret_cast<const H2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+#define IE_HALF_MAX(T, H2, LOW, HIGH)                                             \
+  template <>                                                                     \
+  __device__ __forceinline__ void Max<T>::start(uint4 v) {                        \
+    m = max2<H2>(max2<H2>(v.x, v.y), max2<H2>(v.z, v.w));                         \
+  }                                                                               \
+  template <>                                                                     \
+  __device__ __forceinline__ void Max<T>::add(uint4 v) {                          \
+    m = max2<H2>(m, max2<H2>(max2<H2>(v.x, v.y), max2<H2>(v.z, v.w)));            \
+  }                                                                               \
+  template <>                                                                     \
+  __device__ __forceinline__ float Max<T>::value() const {                        \
+    const H2 p = *reinterpret_cast<const H2*>(&m);                                \
+    return fmaxf(LOW(p), HIGH(p));                                                \
+  }
+IE_HALF_MAX(__nv_bfloat16, __nv_bfloat162, __low2float, __high2float)
+IE_HALF_MAX(__half, __half2, __low2float, __high2float)
+#undef IE_HALF_MAX
+
+// Two f32 in a 64-bit register: one instruction does both.
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 struct Params {
   const void* logits;
   int64_t ld, rows, vocab;
@@ -141,6 +205,30 @@ struct Row {
     nvec = (vocab + off + kPer - 1) / kPer;
   }
   __device__ __forceinline__ int64_t first(int64_t v) const { return v * kPer - off; }
+  // Iteration `it`'s vectors of this thread, packed; -inf where there is no element.
+  __device__ __forceinline__ void load_batch(int64_t it, int64_t end, uint4 (&raw)[kVecs]) const {
+    const int64_t v0 = it * (kThreads * kVecs);
+    const int64_t e0 = first(v0), e1 = first(v0 + kThreads * kVecs);
+    if (v0 + kThreads * kVecs <= end && e0 >= 0 && e1 <= vocab) {
+      const uint4* at = reinterpret_cast<const uint4*>(x + e0) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) raw[i] = __ldg(at + i * kThreads);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int64_t v = v0 + i * kThreads + threadIdx.x, e = first(v);
+        if (v < end && e >= 0 && e + kPer <= vocab) {
+          raw[i] = __ldg(reinterpret_cast<const uint4*>(x + e));
+        } else {
+          T f[kPer];
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            f[j] = v < end && e + j >= 0 && e + j < vocab ? x[e + j] : from_f32<T>(-INFINITY);
+          raw[i] = *reinterpret_cast<const uint4*>(f);
+        }
+      }
+    }
+  }
   __device__ __forceinline__ void load(int64_t v, int64_t end, float (&f)[kPer]) const {
     const int64_t e = first(v);
     if (v < end && e >= 0 && e + kPer <= vocab) {
@@ -159,14 +247,15 @@ token_logprobs_kernel(const Params p) {
   constexpr int kPer = Vec<T>::kPer;
   extern __shared__ uint32_t batch_max[];      // [batches][kThreads], ordered values
   __shared__ uint64_t cand[kCap];
-  __shared__ uint64_t group_key[kGroups];
+  __shared__ uint32_t hits[kCap];              // batches that reach the bound
+  __shared__ __align__(16) uint32_t group_max[kThreads / 2];
   __shared__ uint64_t best[kMaxTop];           // this CTA's list, sorted
   __shared__ uint64_t all_best[kMaxCluster * kMaxTop];   // leader: every CTA's list
   __shared__ Sums all_sums[kMaxCluster];
   __shared__ Sums warp_sums[kWarps];
   __shared__ uint64_t warp_key[kWarps];
-  __shared__ uint64_t thr;
-  __shared__ int count;
+  __shared__ uint32_t bound;
+  __shared__ int n_hits, n_cand;
 
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -181,40 +270,53 @@ token_logprobs_kernel(const Params p) {
 
   Sums mine{-INFINITY, 0.0f, 0.0f};
   uint32_t tmax = 0;       // ordered; 0 is below every value
-  int tbatch = 0;
-  if (tid == 0) count = 0;
+  // the given token's logit arrives meanwhile
+  int64_t token = -1;
+  float given = 0.0f;
+  if (tid == 0) {
+    n_hits = n_cand = 0;
+    token = p.tokens[r];
+    if (token >= 0 && token < p.vocab) given = to_f32<T>(row.x[token]);
+  }
+  uint4 raw[kVecs], ahead[kVecs];
+  if (it0 < it1) row.load_batch(it0, end, ahead);
   for (int64_t it = it0; it < it1; ++it) {
-    const int64_t v0 = it * (kThreads * kVecs) + tid;
-    float f[kVecs][kPer];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) row.load(v0 + i * kThreads, end, f[i]);
-    float bm = f[0][0];
+    for (int i = 0; i < kVecs; ++i) raw[i] = ahead[i];
+    if (it + 1 < it1) row.load_batch(it + 1, end, ahead);
+    Max<T> big;
+    big.start(raw[0]);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) bm = fmaxf(bm, f[i][j]);
+    for (int i = 1; i < kVecs; ++i) big.add(raw[i]);
+    const float bm = big.value();
     if (bm > mine.m) mine = rescaled(mine, bm);
-    const float ref = scaled(mine.m);
-    float s[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
+    const uint64_t ref = f32x2(-scaled(mine.m), -scaled(mine.m));
+    const uint64_t log2e = f32x2(kLog2e, kLog2e);
+    uint64_t s = 0, u = 0;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
+    for (int i = 0; i < kVecs; ++i) {
+      float f[kPer];
+      unpack<T>(raw[i], f);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float d = fmaf(f[i][j], kLog2e, -ref);
-        const float e = ex2(d);
-        s[j & 1] += e;
-        u[j & 1] = fmaf(e, fmaxf(d, kFar), u[j & 1]);
+      for (int j = 0; j < kPer; j += 2) {
+        float d0, d1;
+        unpack2(fma2(f32x2(f[j], f[j + 1]), log2e, ref), d0, d1);
+        const uint64_t e = f32x2(ex2(d0), ex2(d1));
+        s = add2(s, e);
+        u = fma2(e, f32x2(fmaxf(d0, kFar), fmaxf(d1, kFar)), u);
       }
-    mine.s += s[0] + s[1];
-    mine.u += u[0] + u[1];
+    }
+    float lo, hi;
+    unpack2(s, lo, hi);
+    mine.s += lo + hi;
+    unpack2(u, lo, hi);
+    mine.u += lo + hi;
     if (p.top > 0) {
       // a batch past the end holds no element and ranks below every value
+      const int64_t v0 = it * (kThreads * kVecs) + tid;
       const uint32_t o = v0 < end && row.first(v0) < row.vocab ? ordered(bm) : 0u;
       batch_max[(it - it0) * kThreads + tid] = o;
-      if (o > tmax) {
-        tmax = o;
-        tbatch = (int)(it - it0);
-      }
+      tmax = max(tmax, o);
     }
   }
 
@@ -229,72 +331,81 @@ token_logprobs_kernel(const Params p) {
 
   const int top = p.top;
   if (top > 0) {
-    // ---- the threshold: the top-th largest of the group maxima
-    uint64_t k = 0;
-    if (tmax) {          // the first of this thread's elements that holds its maximum
-      const int64_t v0 = (it0 + tbatch) * (kThreads * kVecs) + tid;
-#pragma unroll
-      for (int i = kVecs - 1; i >= 0; --i) {
-        float f[kPer];
-        row.load(v0 + i * kThreads, end, f);
-#pragma unroll
-        for (int j = kPer - 1; j >= 0; --j) {
-          const int64_t e = row.first(v0 + i * kThreads) + j;
-          if (v0 + i * kThreads < end && e >= 0 && e < row.vocab && ordered(f[j]) == tmax)
-            k = ((uint64_t)tmax << 32) | (0xFFFFFFFFu - (uint32_t)e);
+    // ---- the bound: the top-th largest of the maxima of groups of lanes.  Twice as many
+    // groups as wanted leave few elements above it beyond those wanted.
+    const int per_group = top <= 16 ? 8 : top <= 32 ? 4 : 2;
+    uint32_t g = tmax;
+    for (int o = 1; o < per_group; o <<= 1) g = max(g, __shfl_xor_sync(~0u, g, o));
+    if (tid % per_group == 0) group_max[tid / per_group] = g;
+    __syncthreads();
+    const int groups = kThreads / per_group;
+    if (tid < groups) {
+      g = group_max[tid];
+      int above = 0, equal = 0;
+      const uint4* all = reinterpret_cast<const uint4*>(group_max);
+      for (int i = 0; i < groups / 4; ++i) {
+        const uint4 o = all[i];
+        above += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
+        equal += (o.x == g) + (o.y == g) + (o.z == g) + (o.w == g);
+      }
+      if (above < top && above + equal >= top) bound = g;   // all that say so say the same
+    }
+    __syncthreads();
+    const uint32_t reach = max(bound, 1u);       // 0: fewer groups with elements than wanted
+
+    // Collects the elements at or above `from`; false: more than fit.
+    auto collect = [&](uint32_t from) {
+      for (int64_t it = it0; it < it1; ++it)
+        if (batch_max[(it - it0) * kThreads + tid] >= from) {
+          const int at = atomicAdd(&n_hits, 1);
+          if (at < kCap) hits[at] = (uint32_t)((it - it0) * kThreads + tid);
         }
-      }
-    }
-    k = max(k, (uint64_t)__shfl_xor_sync(~0u, k, 1));
-    k = max(k, (uint64_t)__shfl_xor_sync(~0u, k, 2));
-    if ((tid & 3) == 0) group_key[tid >> 2] = k;
-    __syncthreads();
-    {
-      // group g = tid / 4: its rank, counted over a quarter of the groups by each lane
-      int above = 0;
-#pragma unroll 8
-      for (int i = 0; i < kGroups / 4; ++i) {
-        const int g = (tid & 3) + 4 * i;
-        const uint64_t o = group_key[g];
-        above += o > k || (o == k && g < (tid >> 2));   // empty groups share the key 0
-      }
-      above += __shfl_xor_sync(~0u, above, 1);
-      above += __shfl_xor_sync(~0u, above, 2);
-      if ((tid & 3) == 0 && above == top - 1) thr = k;
-    }
-    __syncthreads();
-    // ---- collect every element at or above it
-    const uint64_t floor_key = max(thr, (uint64_t)1);
-    const uint32_t floor_val = (uint32_t)(floor_key >> 32);
-    for (int64_t it = it0; it < it1; ++it) {
-      const uint32_t bm = batch_max[(it - it0) * kThreads + tid];
-      if (bm == 0 || bm < floor_val) continue;
-      const int64_t v0 = it * (kThreads * kVecs) + tid;
-      // among equal values only lower indexes can still enter
-      if (bm == floor_val && row.first(v0) > 0 &&
-          (uint64_t)row.first(v0) > 0xFFFFFFFFu - (uint32_t)floor_key)
-        continue;
-      for (int i = 0; i < kVecs; ++i) {
-        const int64_t v = v0 + i * kThreads;
-        if (v >= end) break;
-        float f[kPer];
-        row.load(v, end, f);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int64_t e = row.first(v) + j;
-          if (e < 0 || e >= row.vocab) continue;
-          const uint64_t ke = key_of(f[j], (uint32_t)e);
-          if (ke >= floor_key) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kCap) cand[at] = ke;
+      __syncthreads();
+      const int n = min(n_hits, kCap);
+      for (int i = warp; i < n; i += kWarps) {      // a warp a batch, a lane an element
+        const int64_t it = it0 + hits[i] / kThreads;
+        const int64_t v = it * (kThreads * kVecs) + hits[i] % kThreads +
+                          (int64_t)(lane / kPer) * kThreads;
+        const int64_t e = row.first(v) + lane % kPer;
+        if (lane < kVecs * kPer && v < end && e >= 0 && e < row.vocab) {
+          const uint32_t o = ordered(to_f32<T>(row.x[e]));
+          if (o >= from) {
+            const int at = atomicAdd(&n_cand, 1);
+            if (at < kCap) cand[at] = ((uint64_t)o << 32) | (0xFFFFFFFFu - (uint32_t)e);
           }
         }
+      }
+      __syncthreads();
+      return n_hits <= kCap && n_cand <= kCap;
+    };
+    bool found = collect(reach);
+    if (!found) {
+      // Many elements equal the bound (a mask's -inf, equal logits): those above it, and as
+      // many that equal it as are wanted, in index order.
+      __syncthreads();
+      if (tid == 0) n_hits = n_cand = 0;
+      __syncthreads();
+      found = collect(reach + 1) && n_cand <= kCap - kThreads - kMaxTop;
+      if (found) {
+        const int above = n_cand;
+        const int64_t e0 = max(row.first(it0 * kThreads * kVecs), (int64_t)0);
+        const int64_t e1 = min(row.first(end), row.vocab);
+        for (int64_t e = e0 + tid; e - tid < e1; e += kThreads) {
+          __syncthreads();
+          if (n_cand - above >= top) break;          // the same for all: nobody adds now
+          __syncthreads();
+          if (e < e1 && ordered(to_f32<T>(row.x[e])) == reach) {
+            const int at = atomicAdd(&n_cand, 1);
+            cand[at] = ((uint64_t)reach << 32) | (0xFFFFFFFFu - (uint32_t)e);
+          }
+        }
+        __syncthreads();
       }
     }
     for (int i = tid; i < top; i += kThreads) best[i] = 0;
     __syncthreads();
-    const int n = count;
-    if (n <= kCap) {
+    const int n = n_cand;
+    if (found) {
       for (int i = tid; i < n; i += kThreads) {
         const uint64_t mykey = cand[i];
         int above = 0;
@@ -302,7 +413,7 @@ token_logprobs_kernel(const Params p) {
         if (above < top) best[above] = mykey;
       }
     } else {
-      // too many elements reach the bound (an adversarial order): one pass per rank
+      // too many elements above the bound (an adversarial order): one pass per rank
       uint64_t below = ~0ull;
       for (int t = 0; t < top; ++t) {
         uint64_t bk = 0;
@@ -354,8 +465,7 @@ token_logprobs_kernel(const Params p) {
   // log sum e^(x - m): the weights' reference is the rounded product m log2 e
   const float logs = (log2s - fmaf(c.m, kLog2e, -scaled(c.m))) * kLn2;
   if (tid == 0) {
-    const int64_t t = p.tokens[r];
-    p.logprobs[r] = t >= 0 && t < p.vocab ? (to_f32<T>(row.x[t]) - c.m) - logs : -INFINITY;
+    p.logprobs[r] = token >= 0 && token < p.vocab ? (given - c.m) - logs : -INFINITY;
     p.entropy[r] = (log2s - c.u / c.s) * kLn2;
   }
   for (int i = tid; i < ranks * top; i += kThreads) {

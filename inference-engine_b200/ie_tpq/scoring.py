@@ -7,9 +7,11 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .device import dtype_code, require_cuda
+from .device import require_cuda
 
-_READY = False
+_DTYPES = {torch.float32: _lib.IE_DT_F32, torch.bfloat16: _lib.IE_DT_BF16,
+           torch.float16: _lib.IE_DT_F16}
+_ENTRY = None      # the library's function, once a GPU has been seen
 
 
 class TokenLogprobs(NamedTuple):
@@ -28,22 +30,26 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     Logits of -inf (a vocabulary mask) are allowed; a row with a NaN or +inf, or
     with no logit above -inf, gives NaN.
     """
-    global _READY
-    if not _READY:
+    global _ENTRY
+    if _ENTRY is None:
         require_cuda()
-        _READY = True
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        _ENTRY = _lib.lib().ie_token_logprobs
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError("logits must be a row-contiguous 2-D tensor")
-    rows, vocab = logits.shape
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {logits.dtype}; expected float32, bfloat16 or float16")
+    rows, vocab = shape
     if tokens.dtype != torch.long or tokens.dim() != 1 or tokens.shape[0] != rows or \
             not tokens.is_contiguous():
         raise ValueError("tokens must be a contiguous int64 tensor of one entry per row")
-    if logits.get_device() < 0 or tokens.get_device() != logits.get_device():
+    index = logits.get_device()
+    if index < 0 or tokens.get_device() != index:
         raise ValueError("logits and tokens must be on one CUDA device")
     if not 0 <= top <= min(vocab, _lib.IE_LOGPROBS_MAX_TOP):
         raise ValueError(f"top={top} outside [0, min({_lib.IE_LOGPROBS_MAX_TOP}, {vocab})]")
-    if logits.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(logits.get_device()):
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top, stream)
     if stream is not None and stream != torch.cuda.current_stream():
         with torch.cuda.stream(stream):   # the outputs belong to that stream
@@ -53,8 +59,8 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     entropy = torch.empty(rows, dtype=f32, device=device)
     top_logprobs = torch.empty(rows, top, dtype=f32, device=device)
     top_tokens = torch.empty(rows, top, dtype=torch.long, device=device)
-    code = _lib.lib().ie_token_logprobs(
-        logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), rows, vocab,
+    code = _ENTRY(
+        logits.data_ptr(), stride[0], _DTYPES[logits.dtype], rows, vocab,
         tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(),
         top_logprobs.data_ptr(), top_tokens.data_ptr(), _lib.stream_ptr())
     if code:
