@@ -308,7 +308,8 @@ int ie_copy_pages(void* const* caches, int32_t ncaches, int64_t page_bytes, int6
                   const int32_t* src, const int32_t* dst, int64_t n, void* stream);
 
 /* ---- log probabilities ----------------------------------------------------------------
- * For each row of logits [rows][vocab] (row stride ld): the log probability of
+ * For each row of logits [rows][vocab] (row stride ld; 0: one row for all): the log
+ * probability of
  * tokens[r] (-inf for a token outside the vocabulary), the entropy in nats, and
  * the `top` largest log probabilities with their tokens, best first, ties to the
  * lower token (top_* may be NULL when top is 0).  Sums are f32.  A row with a

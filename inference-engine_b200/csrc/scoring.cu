@@ -535,8 +535,7 @@ extern "C" int ie_token_logprobs(const void* logits, int64_t ld, int32_t dtype, 
            IE_LOGPROBS_MAX_VOCAB);
   IE_CHECK(top >= 0 && top <= kMaxTop && top <= vocab,
            "token_logprobs: %d alternatives outside [0, min(%d, vocabulary)]", top, kMaxTop);
-  IE_CHECK(ld >= vocab || rows <= 1, "token_logprobs: row stride %lld < vocabulary %lld",
-           (long long)ld, (long long)vocab);
+  IE_CHECK(ld >= 0, "token_logprobs: a row stride of %lld", (long long)ld);
   IE_CHECK(dtype == IE_DT_F32 || dtype == IE_DT_BF16 || dtype == IE_DT_F16,
            "token_logprobs: unsupported dtype %d", dtype);
   if (rows == 0) return IE_OK;

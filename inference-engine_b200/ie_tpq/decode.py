@@ -19,7 +19,8 @@ import numpy as np
 
 @dataclass
 class Layout:
-    """Field-for-field the reference's BatchLayout (ie/core/layout.py:10-45)."""
+    """Field-for-field the reference's BatchLayout (ie/core/layout.py:10-45), and
+    the number of first tokens that all sequences share (the same cache pages)."""
     token_ids: list[int]
     positions: list[int]
     slot_mapping: list[int]
@@ -27,6 +28,7 @@ class Layout:
     query_lens: list[int]
     block_tables: list[list[int]]
     is_prefill: bool
+    shared_prefix_len: int | None = None
 
     @property
     def num_tokens(self) -> int:

@@ -28,6 +28,13 @@ unless ``quantize_lm_head`` (the reference's default, ie/quant/model.py:58-63);
 the dense slice is a plain cuBLAS GEMM.  Sampling runs on the device
 (torch_transformer.py:131-140); under TP the tokens of rank 0 are broadcast
 the same way, so every rank continues with identical tokens.
+
+Layers whose ``config.windows`` entry is not 0 attend with ``window_attention``
+(``config.sinks`` first tokens stay visible), in prefill and decode.  A layout that
+has a ``shared_prefix_len`` (``Layout.shared_prefix_len``, not None) runs its other
+layers on ``shared_prefix_attention``, which reads those first tokens of all
+sequences once.  Both read the cache through the layout's block tables, whose
+entries may be -1 where every layer's window has passed.
 """
 from __future__ import annotations
 
@@ -39,6 +46,7 @@ import numpy as np
 from .attention import (FLASH, PAGED_FLASH_BLOCK, allocate_kv_cache, apply_rope, flash_decode,
                         flash_prefill, paged_attention, rope_write_kv, write_kv)
 from .device import require_cuda
+from .kv_attention import shared_prefix_attention, window_attention
 from .sharding import Shard
 from .tensor_parallel import (ShardedAttention, ShardedMLP, kv_heads_per_rank, quantized_block,
                               rms_norm)
@@ -58,6 +66,10 @@ class DecoderConfig:
     rope_base: float = 500000.0
     norm_eps: float = 1e-5
     rope_halved: bool = False
+    # attention window of each layer (0: the whole context) and the first tokens that stay
+    # visible behind it; None: no layer has one
+    windows: tuple[int, ...] | None = None
+    sinks: int = 0
 
 
 LLAMA3_8B_CONFIG = DecoderConfig(vocab_size=128256, hidden_size=4096, num_layers=32,
@@ -187,6 +199,12 @@ class QuantizedTransformer:
         self.cos = take(source.cos, torch.float32)
         self.sin = take(source.sin, torch.float32)
         self.graphs = None
+        windows = getattr(self.config, "windows", None)
+        if windows is not None and (len(windows) != len(self.attn)
+                                    or any(w < 0 for w in windows)):
+            raise ValueError(f"windows must be {len(self.attn)} sizes of at least 0")
+        self.windows = tuple(windows) if windows is not None else (0,) * len(self.attn)
+        self.sinks = getattr(self.config, "sinks", 0)
         self.num_heads = self.config.num_heads // self.world
         self.num_kv_heads = self.config.num_kv_heads // self.world
 
@@ -211,9 +229,12 @@ class QuantizedTransformer:
         from .linear import qlinear
 
         attn, mlp = self.attn[i], self.mlp[i]
+        paged = plan.get("paged")     # this layer reads the cache with the own kernels
+        own = paged is not None and (self.windows[i] > 0 or paged["prefix"] is not None)
         # A prefill of fresh prompts attends over its own k and v (not the
         # cache) and needs them as tensors; every other step reads the cache.
-        needs_kv = plan["flash"] and layout.is_prefill and plan["paged_tables"] is None
+        needs_kv = (plan["flash"] and layout.is_prefill and plan["paged_tables"] is None
+                    and not own)
         qkv = None if needs_kv else attn.fused_qkv(x)
         if qkv is not None:   # RoPE of q and k and the cache write in one launch
             q = rope_write_kv(qkv, attn.num_heads, attn.num_kv_heads, self.config.head_dim,
@@ -225,7 +246,19 @@ class QuantizedTransformer:
             q = apply_rope(q, positions, self.cos, self.sin, attn.rope_halved)
             k = apply_rope(k, positions, self.cos, self.sin, attn.rope_halved)
             write_kv(k, v, k_cache, v_cache, plan["slots"])
-        if plan["flash"]:
+        if own:
+            lens = dict(cu_seqlens_q=paged["cu_q"], max_query_len=layout.max_query_len,
+                        max_context_len=layout.max_context_len, scale=plan["scale"])
+            if self.windows[i] or not paged["prefix"]:
+                attended = window_attention(q, k_cache, v_cache, paged["tables"],
+                                            paged["context_lens"], block_size,
+                                            window=self.windows[i],
+                                            sinks=self.sinks if self.windows[i] else 0, **lens)
+            else:
+                attended = shared_prefix_attention(q, k_cache, v_cache, paged["tables"],
+                                                   paged["context_lens"], paged["prefix"],
+                                                   block_size, **lens)
+        elif plan["flash"]:
             if layout.is_prefill:
                 attended = flash_prefill(q, k, v, k_cache, v_cache, plan["cu_q"], plan["cu_k"],
                                          layout.max_query_len, layout.max_context_len,
@@ -287,6 +320,15 @@ class QuantizedTransformer:
             "tables32": (block_tables.to(torch.int32)
                          if use_flash and not layout.is_prefill else None),
         }
+        prefix = getattr(layout, "shared_prefix_len", None)
+        if prefix is not None or any(self.windows):
+            plan["paged"] = {
+                "prefix": prefix,
+                "tables": block_tables.to(torch.int32),
+                "context_lens": as_tensor(layout.context_lens, torch.int32),
+                "cu_q": (as_tensor(layout.cu_seqlens_q, torch.int32)
+                         if layout.max_query_len > 1 else None),
+            }
         return self.run(tokens, positions, block_tables, plan, layout, k_caches, v_caches,
                         block_size)
 

@@ -162,6 +162,11 @@ def test_strides_and_alignments(dtype, shift):
     check(big[::2, shift:shift + 1100], t[:3] % 1100, 6)
 
 
+def test_one_row_for_many_tokens():
+    x, t = make(1, 3000, torch.float32, seed=9)
+    check(x.expand(5, -1), torch.arange(5, device="cuda") * 500, 3)
+
+
 def test_streams_and_empty():
     x, t = make(4, 30000, torch.float32, seed=6)
     a = token_logprobs(x, t, top=3)

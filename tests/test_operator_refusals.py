@@ -104,7 +104,7 @@ def logprobs(**kw):
 
 @pytest.mark.parametrize("kw", [
     dict(rows=-1), dict(vocab=0), dict(vocab=2097153, ld=1 << 22), dict(top=65), dict(top=-1),
-    dict(vocab=4, top=5), dict(ld=99), dict(dtype=4), dict(logits=None), dict(tokens=None),
+    dict(vocab=4, top=5), dict(ld=-1), dict(dtype=4), dict(logits=None), dict(tokens=None),
     dict(logprobs=None), dict(entropy=None), dict(top_logprobs=None), dict(top_tokens=None),
     dict(logits=4098)])
 def test_token_logprobs(kw):
