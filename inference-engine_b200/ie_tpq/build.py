@@ -32,7 +32,7 @@ def nvcc() -> str:
 
 
 def command(out: Path) -> list[str]:
-    cmd = [nvcc(), *ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
+    cmd = [nvcc(), "--threads", "0", *ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
            "-shared", "-I", str(REPO / "include"), "-o", str(out)]
     cmd += [str(CSRC / s) for s in SOURCES]
     return cmd
