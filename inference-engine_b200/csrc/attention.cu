@@ -210,13 +210,19 @@ Plan make_plan(const ie_attention_args& a) {
                             : 4;
     plan.decode_per = (int)(ceil_div(ceil_div(own, 64), plan.decode_parts) * 64);
   } else {
-    const int64_t queries = a.max_query_len > 0 ? std::min(a.max_query_len, a.tokens) : a.tokens;
+    // not known: twice the average (the kernel goes on to what lies beyond)
+    const int64_t queries = std::min(
+        a.tokens, a.max_query_len > 0 ? a.max_query_len : 2 * ceil_div(a.tokens, a.seqs));
     plan.twin = queries <= per_tile && own > 128;
     plan.row_tiles = (int)ceil_div(queries, plan.twin ? per_tile : 2 * per_tile);
     // a row tile sees the window of its first token and what lies up to its last
     const int64_t n = a.window > 0 ? std::min(own, seen + 2 * per_tile) : own;
     plan.tile_parts = best_parts(plan.row_tiles * a.seqs * a.kv_heads, n, 128, kSms, 256,
                                  plan.prefix ? 0 : 512);
+    // work items are numbered in 31 bits; the kernel goes on to what lies beyond
+    plan.row_tiles = (int)std::max<int64_t>(
+        1, std::min<int64_t>(plan.row_tiles,
+                             (1ll << 30) / (a.seqs * a.kv_heads * plan.tile_parts)));
     plan.slots = plan.tile_parts * (plan.twin ? 2 : 1);
   }
   if (plan.prefix) plan.slots += plan.prefix_parts * (plan.prefix_twin ? 2 : 1);

@@ -195,9 +195,12 @@ int simt(const Params& p, cudaStream_t s) {
 template <typename T, int NE>
 int join(const Params& p, cudaStream_t s) {
   const int64_t rows = (int64_t)p.tokens * p.heads;
+  // an early launch pays where the join is short; the CTAs of a long one only wait on SMs
+  // that others could use (2048 rows of 18 parts: 30 us with the tiles before it,
+  // 26 without)
   if (rows <= kSms * 8)
     return launch_pdl(attention_join_kernel<T, NE, 4>, rows, 128, 0, s, true, p);
-  return launch_pdl(attention_join_kernel<T, NE, 1>, (rows + 3) / 4, 128, 0, s, true, p);
+  return launch_pdl(attention_join_kernel<T, NE, 1>, (rows + 3) / 4, 128, 0, s, false, p);
 }
 template <typename T>
 int by_size(const Params& p, bool joins, cudaStream_t s) {

@@ -95,9 +95,6 @@ struct Maps {
 };
 
 // ---- PTX ---------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
@@ -145,11 +142,6 @@ __device__ __forceinline__ bool elect() {
       : "=r"(ok)::"memory");
   return ok != 0;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(ok ? 16 : 0)
-               : "memory");
-}
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
@@ -169,11 +161,6 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, 
       " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(u), "r"(bar)
       : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -292,29 +279,6 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// ---- exponentials -----------------------------------------------------------------
-// Two f32 in a 64-bit register: one instruction does both.
-__device__ __forceinline__ uint64_t f32x2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
-  return f32x2(__float_as_uint(lo), __float_as_uint(hi));
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // ---- shared memory -------------------------------------------------------------
 template <int HD>
 struct Layout {
@@ -687,9 +651,6 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
         const int rows = row < 0 ? 0 : min(w.n - (j * kTile + v_lane), a.box);
         const uint32_t ragged = __ballot_sync(~0u, rows > 0 && rows < a.box);
         const int at = rows > 0 ? row : outside;
-        int y[kTile / 8];                 // every lane: the rows of all boxes
-#pragma unroll
-        for (int g = 0; g < kTile / 8; ++g) y[g] = __shfl_sync(~0u, at, g);
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t st = item % L::kStages, bar = smem_u32(&c->full[st]);
@@ -711,24 +672,25 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
           }
           __syncwarp();
           const uint32_t dst = ring + st * L::kTileBytes;
-          if (elect()) {
+#pragma unroll 8
+          for (int g = 0; g < groups; ++g) {
+            const int y = __shfl_sync(~0u, at, g);
+            const int skip = ragged >> g & 1;
+            if (elect()) {
 #pragma unroll
-            for (int g = 0; g < kTile / 8; ++g) {
-              if (g < groups && !(ragged >> g & 1)) {
-#pragma unroll
-                for (int h = 0; h < L::kHalves; ++h)
-                  tma_load(dst + h * 16384 + g * a.box * 128, maps + kv, h * 64, y[g], w.kvh, bar);
-              }
+              for (int h = 0; h < L::kHalves; ++h)
+                if (!skip)
+                  tma_load(dst + h * 16384 + g * a.box * 128, maps + kv, h * 64, y, w.kvh, bar);
             }
           }
           if (ragged) {
             const int g = __ffs(ragged) - 1;      // the last box only
-            const int y0 = __shfl_sync(~0u, row, g), n_rows = __shfl_sync(~0u, rows, g);
+            const int y = __shfl_sync(~0u, row, g), n_rows = __shfl_sync(~0u, rows, g);
             for (int r = 0; r < a.box; ++r)
               if (elect())
                 for (int h = 0; h < L::kHalves; ++h)
                   tma_load(dst + h * 16384 + (g * a.box + r) * 128, maps + 2 + kv, h * 64,
-                           r < n_rows ? y0 + r : outside, w.kvh, bar);
+                           r < n_rows ? y + r : outside, w.kvh, bar);
           }
           __syncwarp();
           ++item;
@@ -1008,7 +970,8 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const uint64_t x = fma2(f32x2(raw[i0 + i], raw[i0 + i + 1]), scale22, ref2);
+            const uint64_t x = fma2(f32x2(__uint_as_float(raw[i0 + i]), __uint_as_float(raw[i0 + i + 1])),
+                                    scale22, ref2);
             float w0, w1;
             unpack2(x, w0, w1);
             w0 = ex2(w0);

@@ -26,6 +26,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace ie {
 namespace score_detail {
@@ -56,11 +57,6 @@ __device__ __forceinline__ float unordered(uint32_t k) {
 }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
   return ((uint64_t)ordered(x) << 32) | (0xFFFFFFFFu - index);
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Sums relative to the maximum m: weights are 2^(x log2 e - scaled(m)).
@@ -158,26 +154,6 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 IE_HALF_MAX(__nv_bfloat16, __nv_bfloat162, __low2float, __high2float)
 IE_HALF_MAX(__half, __half2, __low2float, __high2float)
 #undef IE_HALF_MAX
-
-// Two f32 in a 64-bit register: one instruction does both.
-__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 struct Params {
   const void* logits;
