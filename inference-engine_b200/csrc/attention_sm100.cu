@@ -64,13 +64,12 @@ __device__ uint32_t g_attention_status = 0;
 
 enum Mode { kPrefill = 0, kPrefix = 1 };
 
-// Warps: 0-7 softmax, then the loaders of K and V (one warp with TMA, four that
-// gather), the issuing warp, one or two that load the query rows and the one that
-// fetches the next work item.
+// Warps: 0-7 softmax, then the loaders of K and V (with TMA one of each, as one could not
+// issue the boxes of 16-row pages fast enough; four that gather), the issuing
+// warp and one (gathering: two) for the query rows and the next work item.
 template <bool kTma> struct Warps {
-  static constexpr int kIssue = kTma ? 9 : 12, kQuery = kIssue + 1, kNext = kTma ? 11 : 15;
-  // warps that read the work item: all but the one that fetches it
-  static constexpr int kReaders = kTma ? 11 : 15;
+  static constexpr int kIssue = kTma ? 10 : 12, kQuery = kIssue + 1;
+  static constexpr int kReaders = kTma ? 12 : 15;     // warps that follow the work items
   static constexpr int kThreads = kTma ? 384 : 512;
   // registers of the softmax warps and of the others: together the launch's
   // (384 x 168: 256 x 208 + 128 x 88; 512 x 128: 256 x 192 + 256 x 64)
@@ -346,22 +345,15 @@ struct Items {
     if (elect()) mbar_arrive(smem_u32(&c->next_empty));
   }
 };
-// The warp that takes them over; it never asks again after a refusal.
-__device__ __forceinline__ void next_role(Control* c) {
-  const uint32_t full = smem_u32(&c->next_full);
-  for (uint32_t n = 0;; ++n) {
-    if (n > 0 && !warp_wait(smem_u32(&c->next_empty), (n - 1) & 1, &c->quit)) return;
-    if (elect()) {
-      mbar_expect(full, 16);
-      try_take(smem_u32(c->next), full);
-    }
-    __syncwarp();
-    const long long t0 = clock64();      // what was asked arrives before the CTA ends
-    while (!mbar_try(full, n & 1) && clock64() - t0 < kWaitCycles) {
-    }
-    __syncwarp();
-    if (taken(smem_u32(c->next)) < 0) return;
+// The asking, by one of the readers, once all have read the answer before (`n` asked
+// so far).  A refusal ends the reader's loop: nobody asks again.
+__device__ __forceinline__ void ask_next(Control* c, uint32_t n) {
+  if (n > 0 && !warp_wait(smem_u32(&c->next_empty), (n - 1) & 1, &c->quit)) return;
+  if (elect()) {
+    mbar_expect(smem_u32(&c->next_full), 16);
+    try_take(smem_u32(c->next), smem_u32(&c->next_full));
   }
+  __syncwarp();
 }
 
 // ---- work ------------------------------------------------------------------------
@@ -605,12 +597,13 @@ __device__ void gather_role(const TileParams& a, uint8_t* base, Control* c) {
   flush();
 }
 
-// One warp loads K and V with TMA: boxes of a.box rows (a power of two that divides
-// the page, so a box lies in one page) by 64 elements.  Lane g looks up box g of the
-// tile, one lane issues them all.  A box whose page is not there, and rows past the
-// last key, are read outside the tensor: zeros.
+// One warp loads K (kv 0) or V (kv 1) with TMA: boxes of a.box rows (a power of two that
+// divides the page, so a box lies in one page) by 64 elements.  Lane g looks up box
+// g of the tile, one lane issues them all.  A box whose page is not there, and
+// rows past the last key, are read outside the tensor: zeros.
 template <typename T, int HD>
-__device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* base, Control* c) {
+__device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* base, Control* c,
+                         int kv) {
   using L = Layout<HD>;
   const Params& p = a.p;
   const int lane = threadIdx.x & 31;
@@ -618,7 +611,7 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
   const int v_lane = lane * a.box;         // this lane's box, if lane < groups
   const uint32_t ring = smem_u32(base + L::kRing);
   const int outside = p.cache_rows;
-  uint32_t item = 0;
+  uint32_t item = kv;        // K and V tiles alternate in the ring
 
   for (Items it(blockIdx.x); it.item >= 0; it.next(c)) {
     Work w;
@@ -651,50 +644,48 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
         const int rows = row < 0 ? 0 : min(w.n - (j * kTile + v_lane), a.box);
         const uint32_t ragged = __ballot_sync(~0u, rows > 0 && rows < a.box);
         const int at = rows > 0 ? row : outside;
-#pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t st = item % L::kStages, bar = smem_u32(&c->full[st]);
-          if (item >= L::kStages &&
-              !warp_wait(smem_u32(&c->empty[st]), (item / L::kStages - 1) & 1, &c->quit)) {
-            // what has been started ends before the CTA does
-            const long long t0 = clock64();
-            for (uint32_t i = item - L::kStages; i != item; ++i)
-              while (!mbar_try(smem_u32(&c->full[i % L::kStages]), (i / L::kStages) & 1) &&
-                     clock64() - t0 < kWaitCycles) {
-              }
-            return;
-          }
-          if (lane == 0) {
-            if (kv == 0)
-              *reinterpret_cast<uint4*>(c->invalid[n % kInvalidRing]) =
-                  make_uint4(words[0], words[1], words[2], words[3]);
-            mbar_expect(bar, L::kTileBytes);
-          }
-          __syncwarp();
-          const uint32_t dst = ring + st * L::kTileBytes;
-#pragma unroll 8
-          for (int g = 0; g < groups; ++g) {
-            const int y = __shfl_sync(~0u, at, g);
-            const int skip = ragged >> g & 1;
-            if (elect()) {
-#pragma unroll
-              for (int h = 0; h < L::kHalves; ++h)
-                if (!skip)
-                  tma_load(dst + h * 16384 + g * a.box * 128, maps + kv, h * 64, y, w.kvh, bar);
+        const uint32_t st = item % L::kStages, bar = smem_u32(&c->full[st]);
+        if (item >= L::kStages &&
+            !warp_wait(smem_u32(&c->empty[st]), (item / L::kStages - 1) & 1, &c->quit)) {
+          // what has been started ends before the CTA does
+          const long long t0 = clock64();
+          constexpr uint32_t kBack = L::kStages & ~1;
+          for (uint32_t i = item >= kBack ? item - kBack : kv; i < item; i += 2)
+            while (!mbar_try(smem_u32(&c->full[i % L::kStages]), (i / L::kStages) & 1) &&
+                   clock64() - t0 < kWaitCycles) {
             }
-          }
-          if (ragged) {
-            const int g = __ffs(ragged) - 1;      // the last box only
-            const int y = __shfl_sync(~0u, row, g), n_rows = __shfl_sync(~0u, rows, g);
-            for (int r = 0; r < a.box; ++r)
-              if (elect())
-                for (int h = 0; h < L::kHalves; ++h)
-                  tma_load(dst + h * 16384 + (g * a.box + r) * 128, maps + 2 + kv, h * 64,
-                           r < n_rows ? y + r : outside, w.kvh, bar);
-          }
-          __syncwarp();
-          ++item;
+          return;
         }
+        if (lane == 0) {
+          if (kv == 0)
+            *reinterpret_cast<uint4*>(c->invalid[n % kInvalidRing]) =
+                make_uint4(words[0], words[1], words[2], words[3]);
+          mbar_expect(bar, L::kTileBytes);
+        }
+        __syncwarp();
+        const uint32_t dst = ring + st * L::kTileBytes;
+#pragma unroll 8
+        for (int g = 0; g < groups; ++g) {
+          const int y = __shfl_sync(~0u, at, g);
+          const int skip = ragged >> g & 1;
+          if (elect()) {
+#pragma unroll
+            for (int h = 0; h < L::kHalves; ++h)
+              if (!skip)
+                tma_load(dst + h * 16384 + g * a.box * 128, maps + kv, h * 64, y, w.kvh, bar);
+          }
+        }
+        if (ragged) {
+          const int g = __ffs(ragged) - 1;      // the last box only
+          const int y = __shfl_sync(~0u, row, g), n_rows = __shfl_sync(~0u, rows, g);
+          for (int r = 0; r < a.box; ++r)
+            if (elect())
+              for (int h = 0; h < L::kHalves; ++h)
+                tma_load(dst + h * 16384 + (g * a.box + r) * 128, maps + 2 + kv, h * 64,
+                         r < n_rows ? y + r : outside, w.kvh, bar);
+        }
+        __syncwarp();
+        item += 2;
       }
     }
   }
@@ -711,8 +702,17 @@ __device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t*
   const int t = threadIdx.x & (kQLoaders - 1);
   const int chunk = t % kChunks, r0 = t / kChunks;
   const uint32_t q = smem_u32(base + L::kQ), bar = smem_u32(&c->q_full);
-  uint32_t n = 0;
-  for (Items it(blockIdx.x); it.item >= 0; it.next(c)) {
+  const bool asks = kTma || t < 32;      // one warp asks for the next item
+  uint32_t n = 0, asked = 0;
+  // the next item is asked for after the loads of this one: the wait for the slowest
+  // reader must not hold them up
+  auto next_item = [&](Items& it) {
+    if (asks) ask_next(c, asked++);
+    it.next(c);
+    return it.item >= 0;
+  };
+  Items it(blockIdx.x);
+  do {
     Work w;
     int tile;
     if (!segment(a, it.item, w, tile)) continue;
@@ -750,11 +750,16 @@ __device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t*
         mbar_arrive(bar);
       }
     }
-  }
+  } while (next_item(it));
   // a load that nothing waited for (the others gave up) ends before the CTA does
   if (kTma && c->quit && n > 0) {
     const long long t0 = clock64();
     while (!mbar_try(bar, (n - 1) & 1) && clock64() - t0 < kWaitCycles) {
+    }
+  }
+  if (c->quit && asks && asked > 0) {      // nor does an answer come after it
+    const long long t0 = clock64();
+    while (!mbar_try(smem_u32(&c->next_full), (asked - 1) & 1) && clock64() - t0 < kWaitCycles) {
     }
   }
 }
@@ -1111,14 +1116,12 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::kOtherRegs));
     if (warp < W::kIssue) {
-      if (kTma) tma_role<T, HD>(a, maps.map, base, c);
+      if (kTma) tma_role<T, HD>(a, maps.map, base, c, warp - 8);
       else gather_role<T, HD>(a, base, c);
     } else if (warp == W::kIssue) {
       issue_role<T, HD>(a, base, c, tmem);
     } else if (warp < W::kQuery + (kTma ? 1 : 2)) {
       query_role<T, HD, kTma>(a, &maps.q, base, c);
-    } else if (warp == W::kNext) {
-      next_role(c);
     }
   }
   // every product issued has finished (the softmax warps waited for the last) unless a
