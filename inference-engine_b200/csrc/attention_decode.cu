@@ -348,7 +348,8 @@ template <typename T, int HD, int kWarps, bool kCluster>
 int launch(const Params& p, int per, bool after_tiles, cudaStream_t s) {
   auto kernel = attention_decode_kernel<T, HD, kWarps, kCluster>;
   constexpr int kSmem = smem_bytes<HD, kWarps>();
-  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  static std::atomic<int> allowed[kMaxDevices];
+  if (int rc = allow_smem(kernel, kSmem, allowed)) return rc;
   const int64_t grid = (int64_t)p.seqs * p.kv_heads * ((p.group + 15) / 16) * p.parts;
   if (!kCluster) return launch_pdl(kernel, grid, kWarps * 32, kSmem, s, after_tiles, p, per);
   cudaLaunchConfig_t cfg{};

@@ -1203,8 +1203,8 @@ bool encode(Maps& maps, const Params& p, int dtype, int box) {
 template <typename T, int HD, bool kTma>
 int launch(const TileParams& a, const Maps& maps, cudaStream_t s) {
   auto kernel = attention_tile_kernel<T, HD, kTma>;
-  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   Layout<HD>::kBytes));
+  static std::atomic<int> allowed[kMaxDevices];
+  if (int rc = allow_smem(kernel, Layout<HD>::kBytes, allowed)) return rc;
   const int64_t items = (int64_t)a.row_tiles * a.parts * a.segs * a.p.kv_heads;
   kernel<<<(unsigned)items, Warps<kTma>::kThreads, Layout<HD>::kBytes,
            s>>>(a, maps);

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -36,6 +37,21 @@ inline int launch_status(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)
     return set_error(IE_ERR_CUDA, "launch of %s failed: %s", what, cudaGetErrorString(e));
+  return IE_OK;
+}
+
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device.  The
+// attribute stays with the function, so it is set once for each device and size
+// (`set`: the caller's record for this kernel), not at every launch.
+constexpr int kMaxDevices = 64;
+template <typename K>
+int allow_smem(K* kernel, int bytes, std::atomic<int> (&set)[kMaxDevices]) {
+  int device = 0;
+  IE_CUDA_TRY(cudaGetDevice(&device));
+  const bool known = device >= 0 && device < kMaxDevices;
+  if (known && set[device].load(std::memory_order_relaxed) >= bytes) return IE_OK;
+  IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (known) set[device].store(bytes, std::memory_order_relaxed);
   return IE_OK;
 }
 

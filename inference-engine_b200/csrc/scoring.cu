@@ -474,10 +474,8 @@ int launch(Params p, cudaStream_t s) {
   p.batches = (int)((iters + ranks - 1) / ranks + 1);
   const size_t smem = p.top > 0 ? (size_t)p.batches * kThreads * 4 : 0;
   auto kernel = token_logprobs_kernel<T>;
-  // the attribute is per function and device: set whenever the default is exceeded
-  if (smem > 16 * 1024)
-    IE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)smem));
+  static std::atomic<int> allowed[kMaxDevices];
+  if (int rc = allow_smem(kernel, kMaxBatches * 4 + kThreads * 4, allowed)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.rows * ranks));
   cfg.blockDim = dim3(kThreads);
