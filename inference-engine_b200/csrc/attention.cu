@@ -103,6 +103,7 @@ struct Plan {
   bool twin, prefix_twin;           // row tiles: own keys, shared prefix
   int row_tiles, tile_parts, prefix_row_tiles, prefix_parts;
   int slots;                        // 0: a single part, written to out directly
+  int merge;                        // the decode kernel takes up that many and writes out
 };
 
 // Cost, in keys, of `units` independent rows' worth of n keys in `parts` parts, with
@@ -148,20 +149,18 @@ void choose_decode(const ie_attention_args& a, int64_t units, int64_t own, Plan&
     if (ctas <= 2 * kSms) return std::max(total, cta) + 0.3 * cta;
     return total + (ctas < 3 * kSms ? 0.6 : 0.2) * cta;
   };
-  const bool may_cluster = !plan.prefix;
   double least = cost(1);
   plan.decode_parts = 1;
-  plan.slots = plan.prefix ? 1 : 0;
+  plan.slots = 0;
   const int64_t most = std::min<int64_t>(ceil_div(own, 64), 128);
   for (int64_t parts = 2; parts <= most && units * parts <= 8 * kSms; ++parts) {
-    const double join = plan.prefix ? 16.0 * parts : 400.0 + 16.0 * parts;
+    const double join = 400.0 + 16.0 * parts;
     if (cost(parts) + join < least) {
       least = cost(parts) + join;
       plan.decode_parts = plan.slots = (int)parts;
     }
   }
-  for (int parts = 2; may_cluster && parts <= kMaxDecodeCluster && units * parts <= 2 * kSms;
-       parts *= 2) {
+  for (int parts = 2; parts <= kMaxDecodeCluster && units * parts <= 2 * kSms; parts *= 2) {
     if (cost(parts) + 70 <= least) {
       least = cost(parts) + 70;
       plan.decode_parts = parts;
@@ -225,8 +224,13 @@ Plan make_plan(const ie_attention_args& a) {
                              (1ll << 30) / (a.seqs * a.kv_heads * plan.tile_parts)));
     plan.slots = plan.tile_parts * (plan.twin ? 2 : 1);
   }
-  if (plan.prefix) plan.slots += plan.prefix_parts * (plan.prefix_twin ? 2 : 1);
-  if (plan.slots == 1) plan.slots = 0;
+  if (plan.prefix) {
+    const int prefix_slots = plan.prefix_parts * (plan.prefix_twin ? 2 : 1);
+    if (plan.decode && plan.slots == 0) plan.merge = prefix_slots;
+    plan.slots += prefix_slots;
+  } else if (plan.slots == 1) {
+    plan.slots = 0;
+  }
   return plan;
 }
 
@@ -262,7 +266,10 @@ int run(const ie_attention_args& a, void* workspace, size_t workspace_bytes, con
     }
     if (plan.decode) {
       p.parts = plan.decode_parts;
-      if (int rc = launch_decode(p, a.dtype, plan.decode_per, plan.decode_warps, plan.prefix, s)) return rc;
+      p.merge = plan.merge;
+      if (int rc = launch_decode(p, a.dtype, plan.decode_per, plan.decode_warps, plan.prefix, s))
+        return rc;
+      if (plan.merge) return IE_OK;
     } else if (int rc = launch_tiles(p, a.dtype, false, plan.twin, plan.row_tiles,
                                      plan.tile_parts, s)) {
       return rc;

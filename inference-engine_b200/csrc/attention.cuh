@@ -50,6 +50,7 @@ struct Params {
   float* part_o;
   float2* part_ml;
   int slots, slot0, parts;
+  int merge;       // decode: the parts [0, merge), written by the launch before, join its own
 };
 
 // Cache row of `key`, or -1 when the table names no page of the cache there.
@@ -153,8 +154,9 @@ constexpr int kMaxDecodeCluster = 8;
 // One token per sequence, 16-bit rows of 64 or 128 elements (attention_decode.cu);
 // part i of a row covers its visible keys [i * per, (i + 1) * per), the last one
 // to the end.  Several parts without slots form clusters (at most 8 parts).
-// `after_tiles`: the kernel before on the stream is launch_tiles' of the same call; the
-// two write different slots and run side by side.
+// `after_tiles`: the kernel before on the stream is launch_tiles' of the same call; this
+// one starts beside it and waits for it where it needs its parts (p.merge), or at
+// its end.
 int launch_decode(const Params& p, int dtype, int per, int warps, bool after_tiles,
                   cudaStream_t s);
 // Rows in tiles on the tensor cores (attention_sm100.cu): every sequence's queries

@@ -24,7 +24,10 @@
 // V, the rounding that the tensor cores' operands impose; their sum is not.
 //
 // A few parts of a row form a thread-block cluster and are joined through
-// distributed shared memory: one launch, no workspace.
+// distributed shared memory: one launch, no workspace.  After a shared prefix the
+// kernel runs beside the tiles that compute it, takes up their partial results at
+// its end and writes the finished rows (a launch of its own for that took 10 of 49 us
+// with 64 sequences and 16 parts).
 #include <cooperative_groups.h>
 
 #include "attention.cuh"
@@ -97,6 +100,7 @@ attention_decode_kernel(const Params p, const int per) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_ml[kWarps][16][2];
   __shared__ float2 s_part[16];      // (m, l) of this CTA's part
+  __shared__ float2 s_whole[16];     // merge: the row's reference and its sum
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row_groups = (p.group + 15) / 16;
   int b = blockIdx.x;
@@ -116,7 +120,7 @@ attention_decode_kernel(const Params p, const int per) {
   // The join may be launched.  What it reads is written by this kernel and the one before
   // it: this one ends after both.
   pdl_trigger();
-  if (!kCluster && k0 >= k1) {     // nothing of this row lies in this part
+  if (!kCluster && !p.merge && k0 >= k1) {     // nothing of this row lies in this part
     if (p.slots) {
       if (threadIdx.x < rows)
         p.part_ml[(row0 + threadIdx.x) * p.slots + p.slot0 + part] = make_float2(-INFINITY, 0.0f);
@@ -290,57 +294,126 @@ attention_decode_kernel(const Params p, const int per) {
   __syncthreads();
   const float* all = reinterpret_cast<const float*>(smem);
   float* joined = reinterpret_cast<float*>(smem) + kWarps * 16 * HD;    // cluster: [16][HD]
-  for (int i = threadIdx.x; i < rows * (HD / 2); i += kWarps * 32) {
-    const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
-    float mt = s_ml[0][r][0];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  // (m, l) of row r, and two of its elements relative to 2^m, over the warps of this CTA
+  auto of_warps = [&](int r, int d, float& mt, float& lt, float2& v) {
+    mt = s_ml[0][r][0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) mt = fmaxf(mt, s_ml[w][r][0]);
     const float ref = mt == -INFINITY ? 0.0f : mt;
-    float lt = 0.0f, a = 0.0f, c = 0.0f;
+    lt = 0.0f;
+    v = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = ex2(s_ml[w][r][0] - ref);
-      const float2 v = *reinterpret_cast<const float2*>(all + w * (16 * HD) + r * HD + d);
+      const float2 x = *reinterpret_cast<const float2*>(all + w * (16 * HD) + r * HD + d);
       lt = fmaf(s_ml[w][r][1], f, lt);
-      a = fmaf(v.x, f, a);
-      c = fmaf(v.y, f, c);
+      v.x = fmaf(x.x, f, v.x);
+      v.y = fmaf(x.y, f, v.y);
     }
-    if (kCluster) {
+  };
+  // the same over the CTAs of the cluster, in order
+  auto of_cluster = [&](int r, int d, float& mt, float& lt, float2& v) {
+    mt = -INFINITY;
+    for (int q = 0; q < p.parts; ++q) mt = fmaxf(mt, cluster.map_shared_rank(s_part, q)[r].x);
+    const float ref = mt == -INFINITY ? 0.0f : mt;
+    lt = 0.0f;
+    v = make_float2(0.0f, 0.0f);
+    for (int q = 0; q < p.parts; ++q) {
+      const float2 ml = cluster.map_shared_rank(s_part, q)[r];
+      const float2 x =
+          *reinterpret_cast<const float2*>(cluster.map_shared_rank(joined, q) + r * HD + d);
+      const float f = ex2(ml.x - ref);
+      lt = fmaf(ml.y, f, lt);
+      v.x = fmaf(x.x, f, v.x);
+      v.y = fmaf(x.y, f, v.y);
+    }
+  };
+  auto own = [&](int r, int d, float& mt, float& lt, float2& v) {
+    if (kCluster) of_cluster(r, d, mt, lt, v);
+    else of_warps(r, d, mt, lt, v);
+  };
+  if (kCluster) {
+    for (int i = threadIdx.x; i < rows * (HD / 2); i += kWarps * 32) {
+      const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
+      float mt, lt;
+      float2 v;
+      of_warps(r, d, mt, lt, v);
       if (d == 0) s_part[r] = make_float2(mt, lt);
-      *reinterpret_cast<float2*>(joined + r * HD + d) = make_float2(a, c);
-    } else if (p.slots) {
+      *reinterpret_cast<float2*>(joined + r * HD + d) = v;
+    }
+    cluster.sync();
+  }
+  // ---- the parts of the launch before: their weights, [rows][merge], and the whole sum
+  float* weight = joined + 16 * HD;
+  if (p.merge) {
+    pdl_wait();
+    for (int r = warp; r < rows; r += kWarps) {
+      const float2* ml = p.part_ml + (row0 + r) * p.slots;
+      float mt, lt;
+      float2 v;
+      own(r, 0, mt, lt, v);
+      float top = mt;
+      for (int q = lane; q < p.merge; q += 32) top = fmaxf(top, __ldcg(&ml[q].x));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+      for (int q = lane; q < p.merge; q += 32) {
+        const float2 x = __ldcg(ml + q);
+        const float w = x.y == 0.0f ? 0.0f : ex2(x.x - ref);
+        weight[r * p.merge + q] = w;
+        sum = fmaf(x.y, w, sum);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      if (lane == 0) s_whole[r] = make_float2(ref, fmaf(lt, ex2(mt - ref), sum));
+    }
+    __syncthreads();
+  }
+  // ---- the result; each CTA of a cluster takes its share of the elements
+  const int first = kCluster ? part * (kWarps * 32) : 0;
+  const int stride = kCluster ? p.parts * (kWarps * 32) : kWarps * 32;
+  for (int i = first + threadIdx.x; i < rows * (HD / 2); i += stride) {
+    const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
+    float mt, lt;
+    float2 v;
+    own(r, d, mt, lt, v);
+    if (p.merge) {
+      const float2 whole = s_whole[r];
+      const float f = ex2(mt - whole.x);
+      v.x *= f;
+      v.y *= f;
+      lt = whole.y;
+      constexpr int kAtOnce = 8;
+      const float* src = p.part_o + (row0 + r) * p.slots * HD + d;
+      for (int q0 = 0; q0 < p.merge; q0 += kAtOnce) {
+        float2 x[kAtOnce];
+        float w[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          w[u] = q0 + u < p.merge ? weight[r * p.merge + q0 + u] : 0.0f;
+          x[u] = make_float2(0.0f, 0.0f);
+          if (w[u] != 0.0f)      // 0: nothing was written there
+            x[u] = __ldcg(reinterpret_cast<const float2*>(src + (int64_t)(q0 + u) * HD));
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          v.x = fmaf(x[u].x, w[u], v.x);
+          v.y = fmaf(x[u].y, w[u], v.y);
+        }
+      }
+    }
+    if (p.slots && !p.merge) {
       const int64_t at = (row0 + r) * p.slots + p.slot0 + part;
       if (d == 0) p.part_ml[at] = make_float2(mt, lt);
-      *reinterpret_cast<float2*>(p.part_o + at * HD + d) = make_float2(a, c);
+      *reinterpret_cast<float2*>(p.part_o + at * HD + d) = v;
     } else {
-      store<T>(p, seq, head0 + r, HD, d, a, c, lt);
+      store<T>(p, seq, head0 + r, HD, d, v.x, v.y, lt);
     }
   }
-  if (kCluster) {
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    // each CTA joins its share of the elements, the parts in order
-    for (int i = part * (kWarps * 32) + threadIdx.x; i < rows * (HD / 2);
-         i += p.parts * (kWarps * 32)) {
-      const int r = i / (HD / 2), d = (i % (HD / 2)) * 2;
-      float mt = -INFINITY;
-      for (int q = 0; q < p.parts; ++q) mt = fmaxf(mt, cluster.map_shared_rank(s_part, q)[r].x);
-      const float ref = mt == -INFINITY ? 0.0f : mt;
-      float lt = 0.0f, a = 0.0f, c = 0.0f;
-      for (int q = 0; q < p.parts; ++q) {
-        const float2 x = cluster.map_shared_rank(s_part, q)[r];
-        const float2 v = *reinterpret_cast<const float2*>(
-            cluster.map_shared_rank(joined, q) + r * HD + d);
-        const float f = ex2(x.x - ref);
-        lt = fmaf(x.y, f, lt);
-        a = fmaf(v.x, f, a);
-        c = fmaf(v.y, f, c);
-      }
-      store<T>(p, seq, head0 + r, HD, d, a, c, lt);
-    }
-    cluster.sync();      // the others have read this CTA's part
-  }
+  if (kCluster) cluster.sync();      // the others have read this CTA's part
   pdl_wait();
 }
 
@@ -357,21 +430,23 @@ int launch(const Params& p, int per, bool after_tiles, cudaStream_t s) {
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = p.parts;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_tiles ? 2 : 1;
   IE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, per));
   return IE_OK;
 }
 template <typename T, int HD>
 int launch(const Params& p, int per, int warps, bool after_tiles, cudaStream_t s) {
-  const bool cluster = p.parts > 1 && p.slots == 0;
+  const bool cluster = p.parts > 1 && (p.slots == 0 || p.merge > 0);
   if (cluster)
-    return warps == 8 ? launch<T, HD, 8, true>(p, per, false, s)
-                      : launch<T, HD, 4, true>(p, per, false, s);
+    return warps == 8 ? launch<T, HD, 8, true>(p, per, after_tiles, s)
+                      : launch<T, HD, 4, true>(p, per, after_tiles, s);
   if (warps == 8) return launch<T, HD, 8, false>(p, per, after_tiles, s);
   if (warps == 4) return launch<T, HD, 4, false>(p, per, after_tiles, s);
   return launch<T, HD, 2, false>(p, per, after_tiles, s);
