@@ -3,35 +3,43 @@
 // window and its sinks) and the shared-prefix part of a batch's attention.
 //
 // Rows are (query token, query head of one kv head) pairs, so the heads that
-// share a kv head share its tiles: a tile of 128 rows covers 128 / group
-// tokens.  One CTA per SM, persistent, works on two row tiles at a time
-// ("pair"), or, where there are at most 128 rows, on one row tile whose key
-// tiles alternate between two independent softmax streams ("twin"; the
-// streams are parts of the row's softmax and are joined with the others).  Per tile of
-// 128 keys:
+// share a kv head share its tiles: a row tile is 128 / group whole tokens.  A work
+// item is two row tiles ("pair") or, where one holds all tokens, one row tile
+// whose key tiles alternate between two independent softmax streams ("twin": the
+// streams are parts of the row's softmax, joined with the others).  Per stream
+// and tile of 128 keys:
 //     S = Q K^T     Q, K in shared memory, S in TMEM (f32)
 //     P = 2^(scale2 S - m), rounded to the element type, over S in TMEM
 //     O += P V      P from TMEM, V in shared memory read MN-major, O in TMEM
-// While one stream's softmax runs on its four warps the tensor cores work on
-// the other's products.  The roles: warps 0-3 and 4-7 softmax of the two
-// streams (a row per thread: no shuffles), warps 8-11 load, warp 12 issues.
+// While one stream's softmax runs on its four warps (a row per thread: no
+// shuffles) the tensor cores work on the other's products; the first half of the
+// weights is handed over while the exponentials of the second run.  Two streams
+// are what TMEM holds: S and O of both take its 512 columns.
 //
 // The sinks and the window of a row tile are one run of "virtual" keys (the
-// sinks, then the keys from the first one any row sees), so sinks take a few
-// columns of the first tile instead of a tile of their own, and only tiles at
-// the edges of the mask test their elements.
+// sinks, then the keys from the first one any row sees, both in whole boxes), so
+// sinks take a few columns of the first tile instead of a tile of their own, and
+// only tiles at the edges of the mask test their elements.
 //
-// K and V rows are gathered with cp.async, 16 bytes a lane, straight into the
-// 128-byte-swizzled layout that the MMA descriptors name: pages of any size,
-// one table lookup per key, zeros for rows that are not there.  An arrival on
-// a stage's barrier follows the thread's own wait and a proxy fence, two
-// stages behind the loads.
+// K and V come by TMA in boxes of up to 32 rows, which never cross a page, into the
+// 128-byte-swizzled layout that the MMA descriptors name; pages that no box of 8
+// rows fits are gathered row by row with cp.async.  One CTA per SM; items are
+// taken over with cluster launch control, so the next item's loads run under the
+// end of the last one.
 //
-// Bound by the exponentials as much as by the tensor cores: a 128 x 128 tile
-// costs 1024 cycles of MMA and 16384 exponentials, 1024 cycles of the SM's 16
-// a cycle.  The maximum is raised only when a score passes it by more than
-// 2^8, so the output is rarely rescaled (by its own softmax warps: the product
-// it belongs to has finished by then).
+// What bounds it (2 x 8192 tokens, heads 32/8 x 128, window 2048: 350 us, 1.08 PFLOP/s):
+// a pair of row tiles against a key tile is 2048 cycles of MMA, 2048 of the SM's 16
+// exponentials a cycle, and 256 KB of shared-memory traffic (both products'
+// operands and the loads' writes), 2048 cycles of its 128 bytes: none can hide
+// much of another.  3200 were measured, 2900 with the exponentials left out.  Not
+// kept: a polynomial for a part of the exponentials (slower at every share), two
+// threads a row (registers spill), steps of 64 keys (the products of 64 columns are
+// bound by shared memory).
+//
+// The maximum is raised only when a score passes it by more than 2^8, so the
+// output is rarely rescaled (by its own softmax warps: the product it belongs to has
+// finished by then).  Weights are rounded to the element type, which the MMA's
+// operands have; scores, sums and outputs are f32.
 //
 // A key that some rows of a tile see and others do not enters the others'
 // product with weight 0; a NaN or infinite V there would still poison them.  Rows
