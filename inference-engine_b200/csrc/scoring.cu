@@ -36,8 +36,12 @@ namespace score_detail {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;     // four CTAs an SM: one's selection runs under the others' loads
-constexpr int kWarps = kThreads / 32;
+// Threads of a CTA.  Several CTAs share an SM, so that one's selection runs under the
+// others' loads: four of 256, or eight of 128 where rows are short and the selection
+// weighs more (2304 f16 rows of 8297 with 14 alternatives: 44 us with 256, 30 with
+// 128; 4095 bf16 rows of 20000 with 5: 70 and 48; of 128256 with 1: 189 and 203).
+constexpr int kMany = 256, kFew = 128;
+constexpr int kShortRow = 65536;
 constexpr int kVecs = 4;          // 16-byte vectors of one thread's batch
 constexpr int kMaxTop = IE_LOGPROBS_MAX_TOP;
 constexpr int kCap = 1024;        // collected candidates, and batches to look at
@@ -47,7 +51,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1000.0f;  // 2^kFar == 0: bounds (x - m) where its weight is zero
 
-static_assert(kMaxTop <= kThreads / 2, "the bound is the top-th of the group maxima");
+static_assert(kMaxTop <= kFew, "the bound is the top-th of the group maxima");
 
 // (value, lower index first) as an unsigned key; NaN ranks with -inf.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -171,7 +175,7 @@ struct Params {
 
 // One row as 16-byte vectors from the aligned address at or below its start.
 // A vector that reaches over either end of the row is read element by element.
-template <typename T>
+template <typename T, int kThreads>
 struct Row {
   static constexpr int kPer = Vec<T>::kPer;
   const T* x;
@@ -220,14 +224,15 @@ struct Row {
   }
 };
 
-template <typename T>
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_kernel(const Params p) {
+  constexpr int kWarps = kThreads / 32;
   constexpr int kPer = Vec<T>::kPer;
   extern __shared__ uint32_t batch_max[];      // [batches][kThreads], ordered values
   __shared__ uint64_t cand[kCap];
   __shared__ uint32_t hits[kCap];              // batches that reach the bound
-  __shared__ __align__(16) uint32_t group_max[kThreads / 2];
+  __shared__ __align__(16) uint32_t group_max[kThreads];
   __shared__ uint64_t best[kMaxTop];           // this CTA's list, sorted
   __shared__ uint64_t all_best[kMaxCluster * kMaxTop];   // leader: every CTA's list
   __shared__ Sums all_sums[kMaxCluster];
@@ -241,7 +246,7 @@ token_logprobs_kernel(const Params p) {
   cluster.barrier_arrive();      // every CTA of the row has started before its memory is written
   const int64_t r = blockIdx.x / ranks;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Row<T> row(p, r);
+  const Row<T, kThreads> row(p, r);
   // this CTA's vectors: whole iterations of the row, spread evenly
   const int64_t iters = (row.nvec + kThreads * kVecs - 1) / (kThreads * kVecs);
   const int64_t it0 = iters * rank / ranks, it1 = iters * (rank + 1) / ranks;
@@ -312,7 +317,8 @@ token_logprobs_kernel(const Params p) {
   if (top > 0) {
     // ---- the bound: the top-th largest of the maxima of groups of lanes.  Twice as many
     // groups as wanted leave few elements above it beyond those wanted.
-    const int per_group = top <= 16 ? 8 : top <= 32 ? 4 : 2;
+    int per_group = 1;
+    while (per_group < 8 && kThreads / (2 * per_group) >= 2 * top) per_group *= 2;
     uint32_t g = tmax;
     for (int o = 1; o < per_group; o <<= 1) g = max(g, __shfl_xor_sync(~0u, g, o));
     if (tid % per_group == 0) group_max[tid / per_group] = g;
@@ -463,7 +469,7 @@ token_logprobs_kernel(const Params p) {
   }
 }
 
-template <typename T>
+template <typename T, int kThreads>
 int launch(Params p, cudaStream_t s) {
   constexpr int64_t per_iter = (int64_t)kThreads * kVecs * Vec<T>::kPer;
   const int64_t iters = (p.vocab + Vec<T>::kPer - 1 + per_iter - 1) / per_iter;
@@ -476,7 +482,7 @@ int launch(Params p, cudaStream_t s) {
     ranks *= 2;
   p.batches = (int)((iters + ranks - 1) / ranks + 1);
   const size_t smem = p.top > 0 ? (size_t)p.batches * kThreads * 4 : 0;
-  auto kernel = token_logprobs_kernel<T>;
+  auto kernel = token_logprobs_kernel<T, kThreads>;
   static std::atomic<int> allowed[kMaxDevices];
   if (int rc = allow_smem(kernel, kMaxBatches * 4 + kThreads * 4, allowed)) return rc;
   cudaLaunchConfig_t cfg{};
@@ -493,6 +499,13 @@ int launch(Params p, cudaStream_t s) {
   cfg.numAttrs = 1;
   IE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
   return IE_OK;
+}
+
+template <typename T>
+int launch(const Params& p, cudaStream_t s) {
+  // short rows, and enough of them to fill the SMs with the smaller CTAs
+  return p.vocab <= kShortRow && p.rows >= 148 * 4 ? launch<T, kFew>(p, s)
+                                                   : launch<T, kMany>(p, s);
 }
 
 }  // namespace score_detail
