@@ -180,7 +180,7 @@ Plan make_plan(const ie_attention_args& a) {
   if (!tensor_cores(a) || (per_tile == 0 && (a.cu_seqlens_q || a.prefix_len > 0))) {
     // enough CTAs for every SM's warps, at least 64 keys each
     plan.simt = true;
-    const int64_t rows = a.tokens * a.heads;
+    const int64_t rows = a.tokens * a.kv_heads * ceil_div(group, 8);
     plan.simt_parts = (int)std::max<int64_t>(
         1, std::min({ceil_div(kSms * 16, rows), seen / 64, (int64_t)1024}));
     plan.slots = plan.simt_parts > 1 ? plan.simt_parts : 0;

@@ -1,14 +1,20 @@
 // Paged attention for any element type, head size (up to 256) and alignment, and
 // the joining of partial softmax results.
 //
-// One CTA takes one (query token, head) and one part of the keys that the
-// query sees; its four warps take groups of four keys in turn, lanes across
-// the head size, with the running maximum and sum of a softmax per warp:
-//     m' = max(m, s_j),  l = l 2^(m - m') + sum 2^(s_j - m'),  o likewise,
-// all in f32.  The tensor-core kernels serve 16-bit rows of 64 and 128
-// elements; this kernel serves the rest (f32 models above all), where every
-// query row reads the keys for itself, so it is bound by instruction issue
-// (about 25 instructions a key and warp), not by memory.
+// One CTA takes one query token, up to eight query heads of one kv head and one
+// part of the keys that the query sees, so K and V are read once for those
+// heads.  Its four warps take groups of kKeys keys in turn, lanes across the head
+// size.  The kKeys x kHeads dot products of a group are summed over the lanes
+// together: a butterfly that hands half of the values on at each step ends with one
+// sum a lane after 31 shuffles instead of 5 for each of the 32.  A lane then holds the
+// score of one (head, key), and the softmax's running maximum and sum
+//     m' = max(m, s_j),  l = l 2^(m - m') + sum 2^(s_j - m'),  o likewise
+// are kept per head, all in f32.
+//
+// The tensor-core kernels serve 16-bit rows of 64 and 128 elements; this kernel
+// serves the rest, f32 models above all.  It is bound by instruction issue, about
+// ten instructions a key and head (8 f32 sequences of up to 8192, heads 14/2 x 64:
+// 47 us; 1024 tokens prefilled: 195 us).
 #include "attention.cuh"
 
 namespace ie {
@@ -16,14 +22,39 @@ namespace attn {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kKeys = 4;    // keys a warp takes at once
 
-template <typename T, int NE>
+// v[0 .. N): values of every lane; afterwards the result is the sum over all lanes of
+// v[lane / (32 / N)].
+template <int N>
+__device__ __forceinline__ float sum_lanes(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int n = N / 2, off = 16; off > 0; off >>= 1, n >>= 1) {
+    if (n > 0) {
+      const bool upper = lane & off;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float give = upper ? v[i] : v[i + n], keep = upper ? v[i + n] : v[i];
+        v[i] = keep + __shfl_xor_sync(~0u, give, off);
+      }
+    } else {
+      v[0] += __shfl_xor_sync(~0u, v[0], off);
+    }
+  }
+  return v[0];
+}
+
+template <typename T, int NE, int kHeads>
 __global__ void __launch_bounds__(kWarps * 32)
 attention_simt_kernel(const Params p) {
-  __shared__ float s_ml[kWarps][2];
-  __shared__ float s_o[kWarps][NE * 32];
-  const int t = blockIdx.x, part = blockIdx.y, h = blockIdx.z;
+  constexpr int kKeys = kHeads == 1 ? 8 : 32 / kHeads;    // keys a warp takes at once
+  constexpr int N = kKeys * kHeads, kCopies = 32 / N;     // lanes that hold one score
+  __shared__ float s_ml[kWarps][kHeads][2];
+  __shared__ float s_o[kWarps][kHeads][NE * 32];
+  const int t = blockIdx.x, part = blockIdx.y;
+  const int chunks = (p.group + kHeads - 1) / kHeads;
+  const int kvh = blockIdx.z / chunks, g0 = (blockIdx.z - kvh * chunks) * kHeads;
+  const int h0 = kvh * p.group + g0, heads = min(kHeads, p.group - g0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int seq = sequence_of(p, t);
   const int pos = position_of(p, seq, t);
@@ -31,85 +62,126 @@ attention_simt_kernel(const Params p) {
   // this part of the keys, in whole groups
   const int groups = (keys.n + kKeys - 1) / kKeys;
   const int per = (groups + p.parts - 1) / p.parts * kKeys;
-  const int k0 = min(part * per, keys.n), k1 = min(k0 + per, keys.n);
-  const int kvh = p.group_div.div(h);
+  const int k0 = (int)min((int64_t)part * per, (int64_t)keys.n);
+  const int k1 = (int)min((int64_t)k0 + per, (int64_t)keys.n);
   const int32_t* table = p.tables + (int64_t)seq * p.table_stride;
-  const T* q = static_cast<const T*>(p.q) + t * p.q_token + h * p.q_head;
   const T* kc = static_cast<const T*>(p.k) + kvh * p.head_stride;
   const T* vc = static_cast<const T*>(p.v) + kvh * p.head_stride;
 
-  float qv[NE], o[NE];
+  float q[kHeads][NE], o[kHeads][NE];
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int d = lane + 32 * i;
-    qv[i] = d < p.hd ? to_f32<T>(q[d]) * p.scale2 : 0.0f;
-    o[i] = 0.0f;
-  }
+  for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const int d = lane + 32 * e;
+      q[h][e] = h < heads && d < p.hd
+                    ? to_f32<T>(static_cast<const T*>(
+                          p.q)[t * p.q_token + (h0 + h) * p.q_head + d]) * p.scale2
+                    : 0.0f;
+      o[h][e] = 0.0f;
+    }
+  // of head lane / (kKeys * kCopies); l of this lane's keys alone
   float m = -INFINITY, l = 0.0f;
   for (int j = k0 + warp * kKeys; j < k1; j += kWarps * kKeys) {
-    float s[kKeys];
-    int64_t row[kKeys];
+    // lane i < kKeys looks key i up
+    int slot = -1;
+    if (lane < kKeys && j + lane < k1) {
+      const int key = keys.at(j + lane);
+      slot = cache_slot(p, key < p.prefix ? p.tables : table, key);
+    }
+    const uint32_t there = __ballot_sync(~0u, slot >= 0);
+    if (!there) continue;
+    float s[N];
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) {
-      const int key = keys.at(min(j + i, k1 - 1));
-      const int slot = cache_slot(p, key < p.prefix ? p.tables : table, key);
-      row[i] = j + i < k1 && slot >= 0 ? slot * p.slot_stride : -1;
-      s[i] = 0.0f;
+      const int at = __shfl_sync(~0u, slot, i);
+      float k[NE];
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         const int d = lane + 32 * e;
-        if (row[i] >= 0 && d < p.hd) s[i] = fmaf(qv[e], to_f32<T>(kc[row[i] + d]), s[i]);
+        k[e] = at >= 0 && d < p.hd ? to_f32<T>(kc[at * p.slot_stride + d]) : 0.0f;
+      }
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        float x = q[h][0] * k[0];
+#pragma unroll
+        for (int e = 1; e < NE; ++e) x = fmaf(q[h][e], k[e], x);
+        s[h * kKeys + i] = x;
       }
     }
+    float mine = sum_lanes<N>(s);
+    const int my_key = lane / kCopies % kKeys;
+    const bool seen = there >> my_key & 1;
+    if (!seen) mine = -INFINITY;
+    float mn = mine;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-#pragma unroll
-      for (int i = 0; i < kKeys; ++i) s[i] += __shfl_xor_sync(~0u, s[i], off);
-    float mn = m;
-#pragma unroll
-    for (int i = 0; i < kKeys; ++i)
-      if (row[i] >= 0) mn = fmaxf(mn, s[i]);
+    for (int off = kCopies; off < kKeys * kCopies; off <<= 1)
+      mn = fmaxf(mn, __shfl_xor_sync(~0u, mn, off));
+    mn = fmaxf(mn, m);
     const float ref = mn == -INFINITY ? 0.0f : mn;
-    const float f = ex2(m - ref);
-    m = mn;
-    l *= f;
+    const float f = ex2(m - ref), w = seen ? ex2(mine - ref) : 0.0f;
+    if (__any_sync(~0u, mn > m)) {
 #pragma unroll
-    for (int e = 0; e < NE; ++e) o[e] *= f;
+      for (int h = 0; h < kHeads; ++h) {
+        const float fh = __shfl_sync(~0u, f, h * kKeys * kCopies);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) o[h][e] *= fh;
+      }
+      l *= f;
+      m = mn;
+    }
+    l += w;
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) {
-      if (row[i] < 0) continue;     // not seen: its K and V may hold anything
-      const float w = ex2(s[i] - ref);
-      l += w;
+      if (!(there >> i & 1)) continue;     // not seen: its K and V may hold anything
+      const int at = __shfl_sync(~0u, slot, i);
+      float v[NE];
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         const int d = lane + 32 * e;
-        if (d < p.hd) o[e] = fmaf(w, to_f32<T>(vc[row[i] + d]), o[e]);
+        v[e] = d < p.hd ? to_f32<T>(vc[at * p.slot_stride + d]) : 0.0f;
+      }
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        const float wh = __shfl_sync(~0u, w, (h * kKeys + i) * kCopies);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) o[h][e] = fmaf(wh, v[e], o[h][e]);
       }
     }
   }
-  if (lane == 0) {
-    s_ml[warp][0] = m;
-    s_ml[warp][1] = l;
-  }
+  // a head's sum over its lanes
 #pragma unroll
-  for (int e = 0; e < NE; ++e) s_o[warp][lane + 32 * e] = o[e];
+  for (int off = kCopies; off < kKeys * kCopies; off <<= 1)
+    l += __shfl_xor_sync(~0u, l, off);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (lane == h * kKeys * kCopies) {
+      s_ml[warp][h][0] = m;
+      s_ml[warp][h][1] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s_o[warp][h][lane + 32 * e] = o[h][e];
+  }
   __syncthreads();
-  float mt = s_ml[0][0];
-  for (int w = 1; w < kWarps; ++w) mt = fmaxf(mt, s_ml[w][0]);
-  const float ref = mt == -INFINITY ? 0.0f : mt;
-  float lt = 0.0f;
-  for (int w = 0; w < kWarps; ++w) lt += s_ml[w][1] * ex2(s_ml[w][0] - ref);
-  const int64_t r = (int64_t)t * p.heads + h;
-  const int64_t at = r * p.slots + p.slot0 + part;
-  if (p.slots && threadIdx.x == 0) p.part_ml[at] = make_float2(mt, lt);
-  if (p.slots && lt == 0.0f) return;
-  for (int d = threadIdx.x; d < p.hd; d += kWarps * 32) {
-    float v = 0.0f;
-    for (int w = 0; w < kWarps; ++w) v += s_o[w][d] * ex2(s_ml[w][0] - ref);
-    if (p.slots) p.part_o[at * p.hd + d] = v;
-    else
-      static_cast<T*>(p.out)[t * p.out_token + (int64_t)h * p.hd + d] =
+  for (int i = threadIdx.x; i < heads * p.hd; i += kWarps * 32) {
+    const int h = i / p.hd, d = i - h * p.hd;
+    float mt = s_ml[0][h][0];
+    for (int w = 1; w < kWarps; ++w) mt = fmaxf(mt, s_ml[w][h][0]);
+    const float ref = mt == -INFINITY ? 0.0f : mt;
+    float lt = 0.0f, v = 0.0f;
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(s_ml[w][h][0] - ref);
+      lt = fmaf(s_ml[w][h][1], f, lt);
+      v = fmaf(s_o[w][h][d], f, v);
+    }
+    if (p.slots) {
+      const int64_t at = ((int64_t)t * p.heads + h0 + h) * p.slots + p.slot0 + part;
+      if (d == 0) p.part_ml[at] = make_float2(mt, lt);
+      if (lt != 0.0f) p.part_o[at * p.hd + d] = v;
+    } else {
+      static_cast<T*>(p.out)[t * p.out_token + (int64_t)(h0 + h) * p.hd + d] =
           from_f32<T>(lt == 0.0f ? 0.0f : v / lt);
+    }
   }
 }
 
@@ -186,11 +258,17 @@ attention_join_kernel(const Params p) {
     if (lane + 32 * e < p.hd) out[lane + 32 * e] = from_f32<T>(l == 0.0f ? 0.0f : acc[e] / l);
 }
 
+template <typename T, int NE, int kHeads>
+int simt(const Params& p, cudaStream_t s) {
+  const dim3 grid((unsigned)p.tokens, (unsigned)p.parts,
+                  (unsigned)(p.kv_heads * ((p.group + kHeads - 1) / kHeads)));
+  attention_simt_kernel<T, NE, kHeads><<<grid, kWarps * 32, 0, s>>>(p);
+  return launch_status("attention_simt_kernel");
+}
 template <typename T, int NE>
 int simt(const Params& p, cudaStream_t s) {
-  const dim3 grid((unsigned)p.tokens, (unsigned)p.parts, (unsigned)p.heads);
-  attention_simt_kernel<T, NE><<<grid, kWarps * 32, 0, s>>>(p);
-  return launch_status("attention_simt_kernel");
+  if (p.group == 1) return simt<T, NE, 1>(p, s);
+  return p.group <= 4 ? simt<T, NE, 4>(p, s) : simt<T, NE, 8>(p, s);
 }
 template <typename T, int NE>
 int join(const Params& p, cudaStream_t s) {

@@ -230,6 +230,8 @@ class QuantizedTransformer:
 
         attn, mlp = self.attn[i], self.mlp[i]
         paged = plan.get("paged")     # this layer reads the cache with the own kernels
+        if self.windows[i] and paged is None:
+            raise ValueError("layers with a window need the plan that forward() makes")
         own = paged is not None and (self.windows[i] > 0 or paged["prefix"] is not None)
         # A prefill of fresh prompts attends over its own k and v (not the
         # cache) and needs them as tensors; every other step reads the cache.

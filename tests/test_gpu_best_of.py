@@ -160,3 +160,9 @@ def test_refusals():
         best_of(model, PROMPT, 1, 1, top=301)
     with pytest.raises(ValueError):
         QuantizedTransformer(source((4,), 0), scheme="int8", dtype=torch.float32)
+    windowed = QuantizedTransformer(source((4, 4), 0), scheme="int8", dtype=torch.float32)
+    k, v = windowed.allocate_caches(1, 16)
+    with pytest.raises(ValueError):       # a plan made without the window would ignore it
+        windowed.run(torch.zeros(1, dtype=torch.long, device="cuda"),
+                     torch.zeros(1, dtype=torch.long, device="cuda"), None, {"flash": False},
+                     None, k, v, 16)
