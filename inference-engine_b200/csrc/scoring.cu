@@ -13,19 +13,21 @@
 // unpacking and half of a maximum, two FMAs and an addition on packed pairs, and
 // nothing for the top list; the next batch's loads are in flight meanwhile).  For the list a thread keeps,
 // per batch of four 16-byte vectors, only the batch's largest value in shared
-// memory.  After the pass the largest of every few lanes form groups with distinct
-// elements, so the top-th largest group maximum is a lower bound of the row's
-// top-th element; only batches that reach it are read again (from L2, a warp a
+// memory.  After the pass the lanes of the row form groups with distinct elements
+// (the CTAs of a split row send one another their groups' largest values), so the
+// top-th largest group maximum is a lower bound of the row's top-th element; only batches that reach it are read again (from L2, a warp a
 // batch) and the few elements at or above it are ranked by counting, as 64-bit
 // (value, lower index first) keys.  Where very many equal the bound - a vocabulary
 // mask's -inf, a constant row - those above it are collected and the equal ones
 // taken in index order.  The list does not depend on the order of the atomics.
 //
 // 4095 bf16 rows of 128256 take 187 us with one alternative (5.6 TB/s) and 168 without
-// (6.25 TB/s); 64 f32 rows with 20 take 16 us, one row 7.4.
+// (6.25 TB/s); 64 f32 rows with 20 take 12.7 us, one row 7.4.
 //
 // Few rows are split over a thread-block cluster (up to 8 CTAs a row), merged
-// through distributed shared memory: one launch, no workspace.
+// through distributed shared memory: one launch, no workspace.  With a bound for the
+// row a CTA finds about 2 top / 8 candidates, which its first CTA ranks as they are (a
+// bound and a sorted list per CTA: 64 rows 16.2 us, 16 bf16 rows 11.3 against 7.9).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -51,7 +53,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1000.0f;  // 2^kFar == 0: bounds (x - m) where its weight is zero
 
-static_assert(kMaxTop <= kFew, "the bound is the top-th of the group maxima");
+constexpr int kMaxGroups = 256;
+static_assert(2 * kMaxTop <= kFew && kMany <= kMaxGroups && 4 * kMaxTop <= kMaxGroups,
+              "the bound is the top-th of at least 2 top group maxima");
+static_assert(kMaxCluster * (kMany / 32) <= 64, "one warp merges every warp's sums");
 
 // (value, lower index first) as an unsigned key; NaN ranks with -inf.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -86,6 +91,21 @@ __device__ __forceinline__ Sums merge(Sums a, Sums b) {
   a = rescaled(a, m);
   b = rescaled(b, m);
   return {m, a.s + b.s, a.u + b.u};
+}
+// the sums of all lanes together, in every lane: relative to the largest maximum, then added
+__device__ __forceinline__ Sums warp_merge(Sums a) {
+  a = rescaled(a, unordered(__reduce_max_sync(~0u, ordered(a.m))));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(~0u, a.s, o);
+    a.u += __shfl_xor_sync(~0u, a.u, o);
+  }
+  return a;
+}
+// the same of the first n entries of a shared array, n <= 64, by a whole warp
+__device__ __forceinline__ Sums warp_merge(const Sums* all, int n, int lane) {
+  const Sums none{-INFINITY, 0.0f, 0.0f};
+  return warp_merge(merge(lane < n ? all[lane] : none, lane + 32 < n ? all[lane + 32] : none));
 }
 
 template <typename T> struct Vec {
@@ -232,11 +252,10 @@ token_logprobs_kernel(const Params p) {
   extern __shared__ uint32_t batch_max[];      // [batches][kThreads], ordered values
   __shared__ uint64_t cand[kCap];
   __shared__ uint32_t hits[kCap];              // batches that reach the bound
-  __shared__ __align__(16) uint32_t group_max[kThreads];
-  __shared__ uint64_t best[kMaxTop];           // this CTA's list, sorted
-  __shared__ uint64_t all_best[kMaxCluster * kMaxTop];   // leader: every CTA's list
-  __shared__ Sums all_sums[kMaxCluster];
-  __shared__ Sums warp_sums[kWarps];
+  __shared__ __align__(16) uint32_t group_max[kMaxGroups];   // of the whole row
+  __shared__ uint64_t lists[kMaxCluster * kMaxTop];      // leader: every CTA's candidates
+  __shared__ int counts[kMaxCluster];
+  __shared__ Sums all_sums[kMaxCluster * kWarps];        // leader: every warp's sums
   __shared__ uint64_t warp_key[kWarps];
   __shared__ uint32_t bound;
   __shared__ int n_hits, n_cand;
@@ -304,28 +323,26 @@ token_logprobs_kernel(const Params p) {
     }
   }
 
-  // ---- merged sums of the CTA
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums b{__shfl_xor_sync(~0u, mine.m, o), __shfl_xor_sync(~0u, mine.s, o),
-           __shfl_xor_sync(~0u, mine.u, o)};
-    mine = merge(mine, b);
-  }
-  if (lane == 0) warp_sums[warp] = mine;
+  // ---- every warp's sums to the row's first CTA
+  mine = warp_merge(mine);
+  cluster.barrier_wait();
+  if (lane == 0) *cluster.map_shared_rank(&all_sums[rank * kWarps + warp], 0) = mine;
 
   const int top = p.top;
+  int n = 0;               // candidates of this CTA; all with which the row's list is made
   if (top > 0) {
-    // ---- the bound: the top-th largest of the maxima of groups of lanes.  Twice as many
-    // groups as wanted leave few elements above it beyond those wanted.
+    // ---- the bound: the top-th largest of the maxima of groups of lanes over the row.
+    // Twice as many groups as wanted leave few elements above it beyond those wanted.
     int per_group = 1;
-    while (per_group < 8 && kThreads / (2 * per_group) >= 2 * top) per_group *= 2;
+    while (per_group < 32 && ranks * kThreads / (2 * per_group) >= 2 * top) per_group *= 2;
+    const int mine_of = kThreads / per_group, groups = ranks * mine_of;
     uint32_t g = tmax;
     for (int o = 1; o < per_group; o <<= 1) g = max(g, __shfl_xor_sync(~0u, g, o));
-    if (tid % per_group == 0) group_max[tid / per_group] = g;
-    __syncthreads();
-    const int groups = kThreads / per_group;
-    if (tid < groups) {
-      g = group_max[tid];
+    for (int q = tid % per_group; q < ranks; q += per_group)   // the group's lanes share the CTAs
+      *cluster.map_shared_rank(&group_max[rank * mine_of + tid / per_group], q) = g;
+    if (ranks > 1) cluster.sync(); else __syncthreads();
+    for (int k = tid; k < groups; k += kThreads) {
+      g = group_max[k];
       int above = 0, equal = 0;
       const uint4* all = reinterpret_cast<const uint4*>(group_max);
       for (int i = 0; i < groups / 4; ++i) {
@@ -346,8 +363,8 @@ token_logprobs_kernel(const Params p) {
           if (at < kCap) hits[at] = (uint32_t)((it - it0) * kThreads + tid);
         }
       __syncthreads();
-      const int n = min(n_hits, kCap);
-      for (int i = warp; i < n; i += kWarps) {      // a warp a batch, a lane an element
+      const int hit = min(n_hits, kCap);
+      for (int i = warp; i < hit; i += kWarps) {      // a warp a batch, a lane an element
         const int64_t it = it0 + hits[i] / kThreads;
         const int64_t v = it * (kThreads * kVecs) + hits[i] % kThreads +
                           (int64_t)(lane / kPer) * kThreads;
@@ -387,20 +404,11 @@ token_logprobs_kernel(const Params p) {
         __syncthreads();
       }
     }
-    for (int i = tid; i < top; i += kThreads) best[i] = 0;
-    __syncthreads();
-    const int n = n_cand;
-    if (found) {
-      for (int i = tid; i < n; i += kThreads) {
-        const uint64_t mykey = cand[i];
-        int above = 0;
-        for (int j = 0; j < n; ++j) above += cand[j] > mykey;
-        if (above < top) best[above] = mykey;
-      }
-    } else {
+    n = n_cand;
+    if (!found) {
       // too many elements above the bound (an adversarial order): one pass per rank
       uint64_t below = ~0ull;
-      for (int t = 0; t < top; ++t) {
+      for (n = 0; n < top; ++n) {
         uint64_t bk = 0;
         for (int64_t v = it0 * kThreads * kVecs + tid; v < end; v += kThreads) {
           float f[kPer];
@@ -420,32 +428,37 @@ token_logprobs_kernel(const Params p) {
         __syncthreads();
         bk = warp_key[0];
         for (int w = 1; w < kWarps; ++w) bk = max(bk, warp_key[w]);
-        if (tid == 0) best[t] = bk;
-        below = bk;
         if (bk == 0) break;
+        if (tid == 0) cand[n] = bk;
+        below = bk;
       }
+      __syncthreads();
+    }
+  }
+
+  // ---- the candidates, `top` at most of a CTA, to the row's first CTA
+  if (ranks > 1) {
+    if (tid == 0) *cluster.map_shared_rank(&counts[rank], 0) = min(n, top);
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t k = cand[i];
+      int above = i;
+      if (n > top) {
+        above = 0;
+        for (int j = 0; j < n; ++j) above += cand[j] > k;
+      }
+      if (above < top) *cluster.map_shared_rank(&lists[rank * kMaxTop + above], 0) = k;
+    }
+    cluster.sync();
+    if (rank != 0) return;    // nothing reads a remote CTA's memory after this point
+    n = 0;
+    for (int q = 0; q < ranks; ++q) {
+      if (q % kWarps == warp)
+        for (int i = lane; i < counts[q]; i += 32) cand[n + i] = lists[q * kMaxTop + i];
+      n += counts[q];
     }
   }
   __syncthreads();
-  cluster.barrier_wait();
-
-  // ---- merge the cluster's parts in rank order, on its first CTA
-  if (tid == 0) {
-    Sums c = warp_sums[0];
-    for (int w = 1; w < kWarps; ++w) c = merge(c, warp_sums[w]);
-    *cluster.map_shared_rank(&all_sums[rank], 0) = c;
-  }
-  if (ranks > 1) {
-    for (int i = tid; i < top; i += kThreads)
-      *cluster.map_shared_rank(&all_best[rank * kMaxTop + i], 0) = best[i];
-    cluster.sync();
-    if (rank != 0) return;    // nothing reads a remote CTA's memory after this point
-  } else {
-    for (int i = tid; i < top; i += kThreads) all_best[i] = best[i];
-    __syncthreads();
-  }
-  Sums c = all_sums[0];
-  for (int i = 1; i < ranks; ++i) c = merge(c, all_sums[i]);
+  const Sums c = warp_merge(all_sums, ranks * kWarps, lane);
   const float log2s = log2f(c.s);
   // log sum e^(x - m): the weights' reference is the rounded product m log2 e
   const float logs = (log2s - fmaf(c.m, kLog2e, -scaled(c.m))) * kLn2;
@@ -453,15 +466,10 @@ token_logprobs_kernel(const Params p) {
     p.logprobs[r] = token >= 0 && token < p.vocab ? (given - c.m) - logs : -INFINITY;
     p.entropy[r] = (log2s - c.u / c.s) * kLn2;
   }
-  for (int i = tid; i < ranks * top; i += kThreads) {
-    const uint64_t k = all_best[(i / top) * kMaxTop + i % top];
-    if (k == 0) continue;
-    int above = i;
-    if (ranks > 1) {
-      above = 0;
-      for (int q = 0; q < ranks; ++q)
-        for (int j = 0; j < top; ++j) above += all_best[q * kMaxTop + j] > k;
-    }
+  for (int i = tid; i < n; i += kThreads) {
+    const uint64_t k = cand[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += cand[j] > k;
     if (above < top) {
       p.top_logprobs[r * top + above] = (unordered((uint32_t)(k >> 32)) - c.m) - logs;
       p.top_tokens[r * top + above] = (int64_t)(0xFFFFFFFFu - (uint32_t)k);

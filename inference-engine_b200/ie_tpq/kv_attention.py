@@ -98,7 +98,7 @@ def _attend(name, q, k_cache, v_cache, block_tables, context_lens, block_size, w
                            max_context_len, scale, out, None)
 
     if out is None:
-        out = torch.empty(tokens, heads, head_dim, dtype=dtype, device=q.device)
+        out = q.new_empty(tokens, heads, head_dim)
     try:
         args = _ARGS.pack(
             q.data_ptr(), q_stride[0], q_stride[1], k_cache.data_ptr(), v_cache.data_ptr(),
@@ -109,7 +109,7 @@ def _attend(name, q, k_cache, v_cache, block_tables, context_lens, block_size, w
     except struct.error as exc:
         raise ValueError(f"{name[3:]}: {exc}") from exc
     need = _entry("ie_attention_workspace_size")(args)
-    workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    workspace = q.new_empty(need, dtype=torch.uint8) if need else None
     code = entry(args, workspace.data_ptr() if need else None, need, _lib.stream_ptr())
     if code:
         _lib.check(code, name[3:])

@@ -54,11 +54,10 @@ def token_logprobs(logits, tokens, top: int = 0, stream=None) -> TokenLogprobs:
     if stream is not None and stream != torch.cuda.current_stream():
         with torch.cuda.stream(stream):   # the outputs belong to that stream
             return token_logprobs(logits, tokens, top)
-    f32, device = torch.float32, logits.device
-    logprobs = torch.empty(rows, dtype=f32, device=device)
-    entropy = torch.empty(rows, dtype=f32, device=device)
-    top_logprobs = torch.empty(rows, top, dtype=f32, device=device)
-    top_tokens = torch.empty(rows, top, dtype=torch.long, device=device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    entropy = logprobs.new_empty(rows)
+    top_logprobs = logprobs.new_empty(rows, top)
+    top_tokens = tokens.new_empty(rows, top)
     code = _ENTRY(
         logits.data_ptr(), stride[0], _DTYPES[logits.dtype], rows, vocab,
         tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(),

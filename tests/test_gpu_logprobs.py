@@ -149,6 +149,20 @@ def test_not_finite():
             assert torch.equal(a[r], b[r])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("part", [0, 5, 7])
+def test_one_part_holds_the_allowed_tokens(dtype, part):
+    """A split row whose other parts are all masked, and one whose parts all hold less
+    than the wanted number."""
+    x, t = make(2, 128000, dtype, seed=part)
+    x[0, :part * 16000] = float("-inf")
+    x[0, (part + 1) * 16000:] = float("-inf")
+    x[1] = float("-inf")
+    x[1, part::16000] = torch.arange(8, device="cuda").to(dtype)
+    check(x, t, 20)
+    check(x, t, 64)
+
+
 def test_tokens_outside_the_vocabulary():
     x, _ = make(4, 100, torch.float32)
     check(x, torch.tensor([-1, 100, 2 ** 40, 99], device="cuda"), 1)
