@@ -128,45 +128,68 @@ int best_parts(int64_t units, int64_t n, int64_t step, int wide, int64_t fixed, 
   return (int)best;
 }
 
+// Whether the CTAs of the decode kernel, one an SM with eight warps, all start at once.  A
+// cluster lies in one GPC: 14 of eight CTAs fit (16 with eight warps each ran in two
+// rounds: 2 sequences of 660, 10.8 us; with four, two CTAs an SM, 6.2), and 34 of four
+// (36: 10.6 us and 8.3).
+bool eight_warps(int64_t ctas, int64_t cluster) {
+  return ctas <= (cluster == 8 ? 14 * 8 : cluster == 4 ? 34 * 4 : kSms);
+}
+
 // Parts of the decode kernel's rows and how they are joined.  Times are counted in
 // keys of one CTA of four warps (13 ns on B200 for heads of 128), fitted to
 // measurements over 1 to 64 sequences of 512 to 65536 keys:
 //   - 160 such CTAs draw all of HBM; a batch's contexts are taken to be 0.7 of the
 //     longest on average;
-//   - up to 148 CTAs have eight warps and take 0.65 of the time; the next 148 share
-//     SMs;
+//   - up to 148 CTAs (see eight_warps) have eight warps and take 0.65 of the time; the
+//     next 148 share SMs;
 //   - within one round of CTAs the longest part ends it (0.3 for uneven lengths),
 //     a second round that is short of half costs 0.6 of a CTA, and with more
 //     rounds the scheduler evens the lengths out (0.2);
+//   - of a batch's parts 0.7 have keys, and where only two CTAs share an SM (heads of
+//     128) their second round costs 0.9 (2 sequences of 20000, 8 kv heads: 20 parts
+//     29.9 us, 24 31.7, 28 41, 32 37);
 //   - a start costs 96, a join within a cluster 70, a joining launch 400 and 16 a
 //     part.
 void choose_decode(const ie_attention_args& a, int64_t units, int64_t own, Plan& plan) {
   const double total = (a.seqs == 1 ? 1.0 : 0.7) * (double)(units * own) / 160;
-  auto cost = [&](int64_t parts) {
+  auto cost = [&](int64_t parts, int64_t cluster) {
     const int64_t ctas = units * parts;
     const double cta = (double)(ceil_div(ceil_div(own, 64), parts) * 64 + 96) *
-                       (ctas <= kSms ? 0.65 : 1.0);
+                       (eight_warps(ctas, cluster) ? 0.65 : 1.0);
     if (ctas <= 2 * kSms) return std::max(total, cta) + 0.3 * cta;
-    return total + (ctas < 3 * kSms ? 0.6 : 0.2) * cta;
+    if (parts == 1 || a.seqs == 1 || a.head_dim < 128) return total + (ctas < 3 * kSms ? 0.6 : 0.2) * cta;
+    const double busy = 0.7 * (double)ctas;
+    return busy <= 2 * kSms ? std::max(total, cta) + 0.3 * cta
+                            : total + (busy < 4 * kSms ? 0.9 : 0.2) * cta;
   };
-  double least = cost(1);
+  double least = cost(1, 1);
   plan.decode_parts = 1;
   plan.slots = 0;
   const int64_t most = std::min<int64_t>(ceil_div(own, 64), 128);
   for (int64_t parts = 2; parts <= most && units * parts <= 8 * kSms; ++parts) {
     const double join = 400.0 + 16.0 * parts;
-    if (cost(parts) + join < least) {
-      least = cost(parts) + join;
+    if (cost(parts, 1) + join < least) {
+      least = cost(parts, 1) + join;
       plan.decode_parts = plan.slots = (int)parts;
     }
   }
   for (int parts = 2; parts <= kMaxDecodeCluster && units * parts <= 2 * kSms; parts *= 2) {
-    if (cost(parts) + 70 <= least) {
-      least = cost(parts) + 70;
+    if (cost(parts, parts) + 70 <= least) {
+      least = cost(parts, parts) + 70;
       plan.decode_parts = parts;
       plan.slots = 0;
     }
   }
+}
+
+// A short prefix of few sequences: the decode kernel reads it for each of them, from L2
+// after the first, and the tiles' launch and the parts' round trip are saved.  32/8 heads
+// of 128, 60 keys of their own, us in one pass and in two: 4 sequences on 64: 4.5 and
+// 10.3, on 1024: 8.0 and 10.8, on 4096: 13.8 and 14.8, 16 on 1024: 13.5 and 13.8; beyond the
+// bound 8 on 4096: 21.2 and 15.2, 32 on 1024: 19.9 and 16.8.
+bool prefix_in_decode(const ie_attention_args& a, int64_t units) {
+  return !a.cu_seqlens_q && units * a.prefix_len <= 160 * 1024;
 }
 
 Plan make_plan(const ie_attention_args& a) {
@@ -186,24 +209,25 @@ Plan make_plan(const ie_attention_args& a) {
     plan.slots = plan.simt_parts > 1 ? plan.simt_parts : 0;
     return plan;
   }
-  plan.prefix = a.prefix_len > 0;
+  // (without cu_seqlens_q) the decode kernel's rows
+  const int64_t units = a.seqs * a.kv_heads * ceil_div(group, 16);
+  plan.prefix = a.prefix_len > 0 && !prefix_in_decode(a, units);
   if (plan.prefix) {
     plan.prefix_twin = a.tokens <= per_tile;
     plan.prefix_row_tiles = (int)ceil_div(a.tokens, plan.prefix_twin ? per_tile : 2 * per_tile);
     plan.prefix_parts = best_parts(plan.prefix_row_tiles * a.kv_heads, a.prefix_len, 128, kSms,
                                    256, 512);
   }
-  const int64_t own = std::max<int64_t>(1, seen - a.prefix_len);
+  const int64_t own = std::max<int64_t>(1, plan.prefix ? seen - a.prefix_len : seen);
   if (!a.cu_seqlens_q) {
     plan.decode = true;
-    const int64_t units = a.seqs * a.kv_heads * ceil_div(group, 16);
     choose_decode(a, units, own, plan);
     const int64_t ctas = units * plan.decode_parts;
     // Eight warps an SM, as one CTA or two.  Rows that a window makes equally long also
     // fill one round of four (64 sequences, window 4096: 151 us against 157; uneven
     // ones lose: 32 sequences of up to 32768 448 against 356).
     const bool even = a.window > 0 && a.window + a.sinks < keys;
-    plan.decode_warps = ctas <= kSms ? 8
+    plan.decode_warps = eight_warps(ctas, plan.slots ? 1 : plan.decode_parts) ? 8
                         : even && plan.decode_parts == 1 && ctas > 2 * kSms && ctas <= 4 * kSms
                             ? 2
                             : 4;

@@ -159,7 +159,9 @@ attention_decode_kernel(const Params p, const int per) {
   // the cache row of key lane % 16 of this warp's step i (-1: not seen)
   auto slot_of = [&](int i) {
     const int key = k0 + (i * kWarps + warp) * kStep + (lane & 15);
-    return i < mine && key < k1 ? cache_slot(p, table, keys.at(key)) : -1;
+    if (i >= mine || key >= k1) return -1;
+    const int at = keys.at(key);
+    return cache_slot(p, at < p.prefix ? p.tables : table, at);
   };
   auto load = [&](int i, int slot) {
     const uint32_t dst = ring + (i % kStages) * (2 * kTile);
