@@ -25,8 +25,9 @@
 // V, the rounding that the tensor cores' operands impose; their sum is not.
 //
 // A few parts of a row form a thread-block cluster and are joined through
-// distributed shared memory: one launch, no workspace.  After a shared prefix the
-// kernel runs beside the tiles that compute it, takes up their partial results at
+// distributed shared memory: one launch, no workspace.  A short prefix that the
+// sequences share is read for each of them, through the first table row.  After a longer
+// one the kernel runs beside the tiles that compute it, takes up their partial results at
 // its end and writes the finished rows (a launch of its own for that took 10 of 49 us
 // with 64 sequences and 16 parts).
 #include <cooperative_groups.h>

@@ -42,6 +42,41 @@ def test_batch_sizes(seqs):
     check(Batch([140 + i for i in range(seqs)], 8, 2, 64, F16, 16, prefix=130, seed=seqs))
 
 
+# rows (sequences times kv heads) times prefix beyond what the decode kernel takes on alone
+@pytest.mark.parametrize("seqs,heads,kv,hd,dtype,prefix", [
+    (24, 32, 8, 128, BF16, 901), (24, 64, 8, 128, F16, 1100), (90, 14, 2, 64, F16, 1000),
+    (90, 8, 2, 64, BF16, 928), (3, 8, 8, 128, BF16, 8191), (9, 34, 2, 64, F16, 5000)])
+@pytest.mark.parametrize("own", [1, 40, 700])
+def test_prefix_beyond_one_launch(seqs, heads, kv, hd, dtype, prefix, own):
+    lens = [prefix + 1 + (i * 37) % own for i in range(seqs)]
+    lens[1], lens[2] = prefix - 3, 0        # one shorter than the prefix, one empty
+    b = Batch(lens, heads, kv, hd, dtype, 16, prefix=prefix, seed=own)
+    got = check(b)
+    assert torch.count_nonzero(got[2]) == 0
+    assert torch.equal(check(b), got)
+
+
+def test_prefix_beyond_one_launch_in_a_graph_and_beside_a_nan():
+    b = Batch([1000 + i for i in range(24)], 32, 8, 128, BF16, 16, prefix=1000, seed=12)
+    b.ctx[0] = 500
+    call = lambda: shared_prefix_attention(b.q, b.k, b.v, b.tables, b.ctx, 1000, 16, **b.lens())
+    want = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    graph.replay()
+    assert torch.equal(out, want)
+    b.v[int(b.tables[0, 50]) * 16] = float("nan")      # position 800
+    graph.replay()
+    assert torch.equal(out[0], want[0])                 # its context ends before
+    assert torch.isnan(out[1:]).all()
+
+
 @pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16), (64, F32)])
 def test_several_queries(hd, dtype):
     query = [1, 7, 40, 0, 3]
