@@ -264,7 +264,7 @@ int ie_rope_kv(const void* qkv, int64_t ld_qkv, int32_t dtype, int64_t tokens, i
  * (window == 0 or j > p - window or j < sinks).
  * ie_shared_prefix_attention: j <= p, where the keys below prefix_len are the
  * same for every sequence and are looked up in the FIRST row of block_tables;
- * they are read once for the whole batch.
+ * they are read once for the whole batch (a short prefix once a sequence, from L2).
  *
  * Both: a query that sees nothing (an empty context) gets zeros.  A key whose
  * table entry names no page of the cache (-1, as a page given back reads) is not
@@ -284,7 +284,7 @@ typedef struct ie_attention_args {
   const int32_t* cu_seqlens_q;              /* [seqs + 1], in device memory, or NULL */
   void* out;                                /* [tokens][heads][head_dim] of q's type */
   int64_t out_token_stride;
-  int64_t tokens, seqs;
+  int64_t tokens, seqs;                     /* tokens * heads < 2^24, seqs * heads < 2^23 */
   int64_t max_query_len, max_context_len;   /* the longest of the batch (0: not known): they
                                                size the launch, any value gives the result */
   int64_t window, sinks, prefix_len;

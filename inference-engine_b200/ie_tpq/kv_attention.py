@@ -142,8 +142,8 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, pre
                             max_context_len: int = 0, scale: float | None = None, out=None,
                             stream=None):
     """Causal attention of sequences that begin with the same ``prefix_len`` tokens:
-    the prefix is read once for the whole batch, through the first row of
-    ``block_tables``, and the keys from ``prefix_len`` on through each
+    the prefix is read through the first row of ``block_tables``, once for the
+    whole batch (a short prefix of few sequences: by each, from L2), and the keys from ``prefix_len`` on through each
     sequence's own row.  A sequence shorter than the prefix sees its part of
     it.  The other arguments are those of ``window_attention``."""
     return _attend("ie_shared_prefix_attention", q, k_cache, v_cache, block_tables, context_lens,

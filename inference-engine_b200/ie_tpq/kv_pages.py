@@ -149,7 +149,7 @@ class KVPagePool:
 
     def free(self, seqs) -> None:
         """Gives the sequences' pages back (those that no other sequence shares)."""
-        seqs = [seqs] if isinstance(seqs, int) else list(seqs)
+        seqs = list(seqs) if hasattr(seqs, "__iter__") else [seqs]
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence is freed once")
         for s in [self._sequence(n) for n in seqs]:
