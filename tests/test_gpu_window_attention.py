@@ -4,10 +4,13 @@ sinks around their edges, pages that end inside a tile, rows that see nothing,
 NaN where nothing may be read, strides, streams and refusals."""
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
+from ie_tpq import _lib
 from ie_tpq.kv_attention import window_attention
 from tests.attention_oracle import Batch, as_f64, assert_close, attention
 
@@ -267,3 +270,52 @@ def test_refusals():
     with pytest.raises(ValueError):
         window_attention(big, big.expand(16, 2, 512).contiguous(),
                          big.expand(16, 2, 512).contiguous(), b.tables[:1], b.ctx[:1], 16)
+
+
+def c_args(b, out, window=0, sinks=0, prefix=0):
+    a = _lib.AttentionArgs()
+    a.q, a.q_token_stride, a.q_head_stride = b.q.data_ptr(), b.q.stride(0), b.q.stride(1)
+    a.k_cache, a.v_cache, a.cache_slots = b.k.data_ptr(), b.v.data_ptr(), b.k.shape[0]
+    a.slot_stride, a.head_stride = b.k.stride(0), b.k.stride(1)
+    a.block_tables, a.table_stride, a.table_width = (b.tables.data_ptr(), b.tables.stride(0),
+                                                     b.tables.shape[1])
+    a.context_lens = b.ctx.data_ptr()
+    a.cu_seqlens_q = None if b.cu is None else b.cu.data_ptr()
+    a.out, a.out_token_stride = out.data_ptr(), out.stride(0)
+    a.tokens, a.seqs = b.q.shape[0], len(b.context)
+    lens = b.lens()
+    a.max_query_len, a.max_context_len = lens["max_query_len"], lens["max_context_len"]
+    a.window, a.sinks, a.prefix_len = window, sinks, prefix
+    a.dtype = {BF16: _lib.IE_DT_BF16, F16: _lib.IE_DT_F16, F32: _lib.IE_DT_F32}[b.q.dtype]
+    a.heads, a.kv_heads, a.head_dim = b.q.shape[1], b.k.shape[1], b.q.shape[2]
+    a.block_size, a.scale = b.block, b.q.shape[2] ** -0.5
+    return a
+
+
+@pytest.mark.parametrize("case", ["split", "twin", "decode", "prefix", "f32"])
+def test_a_workspace_needs_16_bytes_of_alignment(case):
+    """The parts of split rows in a workspace that starts 16 bytes past a 32-byte boundary."""
+    entry, prefix = "ie_window_attention", 0
+    if case == "split":
+        b = Batch([2000], 4, 1, 128, BF16, 16, query=[300], seed=20)
+    elif case == "twin":
+        b = Batch([1500, 700], 4, 2, 64, F16, 16, query=[5, 9], seed=21)
+    elif case == "decode":
+        b = Batch([20001], 2, 1, 128, BF16, 16, seed=22)
+    elif case == "prefix":
+        entry, prefix = "ie_shared_prefix_attention", 901
+        b = Batch([901 + i for i in range(24)], 32, 8, 128, BF16, 16, prefix=901, seed=23)
+    else:
+        b = Batch([3000, 500], 4, 2, 64, F32, 16, seed=24)
+    out = torch.full_like(b.q, float("nan"))
+    a = c_args(b, out, prefix=prefix)
+    need = _lib.lib().ie_attention_workspace_size(ctypes.byref(a))
+    assert need > 0
+    room = torch.empty(need + 64, dtype=torch.uint8, device="cuda")
+    assert room.data_ptr() % 32 == 0
+    for offset in (0, 16):
+        out.fill_(float("nan"))
+        _lib.check(getattr(_lib.lib(), entry)(ctypes.byref(a), room.data_ptr() + offset, need,
+                                              _lib.stream_ptr()))
+        want, weight, largest = b.oracle(prefix=prefix)
+        assert_close(out, want, weight, largest, b.q.shape[2])
