@@ -258,8 +258,13 @@ Plan make_plan(const ie_attention_args& a) {
   return plan;
 }
 
+// The workspace: the parts' sums in f32, then their (m, l) pairs, which start on an
+// 8-byte boundary whatever the head size.
+size_t part_sums(const ie_attention_args& a, int slots) {
+  return ((size_t)a.tokens * a.heads * slots * a.head_dim + 1) / 2 * 2;
+}
 size_t part_bytes(const ie_attention_args& a, int slots) {
-  return (size_t)a.tokens * a.heads * slots * (a.head_dim * 4 + 8);
+  return part_sums(a, slots) * 4 + (size_t)a.tokens * a.heads * slots * 8;
 }
 
 int run(const ie_attention_args& a, void* workspace, size_t workspace_bytes, const char* who,
@@ -273,8 +278,7 @@ int run(const ie_attention_args& a, void* workspace, size_t workspace_bytes, con
   p.prefix = (int)std::min<int64_t>(a.prefix_len, 0x7FFFFFFF);
   p.slots = plan.slots;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)a.tokens * a.heads * plan.slots *
-                                                       a.head_dim);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + part_sums(a, plan.slots));
   if (plan.simt) {
     p.parts = plan.simt_parts;
     if (int rc = launch_simt(p, a.dtype, s)) return rc;

@@ -319,3 +319,14 @@ def test_a_workspace_needs_16_bytes_of_alignment(case):
                                               _lib.stream_ptr()))
         want, weight, largest = b.oracle(prefix=prefix)
         assert_close(out, want, weight, largest, b.q.shape[2])
+
+
+@pytest.mark.parametrize("hd", [1, 33, 127, 255])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_odd_head_sizes_split_into_parts(hd, dtype):
+    for query in (None, [3]):
+        b = Batch([200], 1, 1, hd, dtype, 16, query=query, seed=hd)
+        out = torch.empty_like(b.q)
+        assert _lib.lib().ie_attention_workspace_size(ctypes.byref(c_args(b, out))) > 0
+        check(b)
+        check(b, window=150, sinks=3)

@@ -61,6 +61,16 @@ def test_workspace_that_is_missing_or_small():
     assert lib.ie_window_attention(None, None, 0, None) == _lib.IE_ERR_INVALID
 
 
+@pytest.mark.parametrize("head_dim", [1, 33, 255])
+def test_odd_head_sizes_leave_room_for_aligned_pairs(head_dim):
+    """The parts' (m, l) pairs follow an odd number of f32 sums on an 8-byte boundary."""
+    a = args(tokens=1, seqs=1, heads=1, kv_heads=1, head_dim=head_dim, q_token_stride=head_dim,
+             q_head_stride=head_dim, out_token_stride=head_dim, slot_stride=head_dim,
+             head_stride=head_dim, dtype=_lib.IE_DT_F32, table_width=12, table_stride=12)
+    need = _lib.lib().ie_attention_workspace_size(ctypes.byref(a))     # three parts
+    assert need == (3 * head_dim + 1) * 4 + 3 * 8
+
+
 def test_nothing_to_do_is_not_an_error():
     a = args(tokens=0, seqs=0)
     assert _lib.lib().ie_window_attention(ctypes.byref(a), None, 0, None) == _lib.IE_OK
