@@ -15,9 +15,10 @@ int validate(const ie_attention_args& a, const char* who) {
            "%s: %d query heads over %d kv heads", who, a.heads, a.kv_heads);
   IE_CHECK(a.head_dim > 0 && a.head_dim <= IE_ATTENTION_MAX_HEAD_DIM,
            "%s: a head size of %d outside [1, %d]", who, a.head_dim, IE_ATTENTION_MAX_HEAD_DIM);
-  // the launches number (token, head, part) and (row tile, head, part) in 31 bits
-  IE_CHECK(a.tokens >= 0 && a.tokens * a.heads < (1ll << 31) / 128, "%s: %lld query tokens", who,
-           (long long)a.tokens);
+  // the launches number (token, head, part) and (row tile, head, part) in 31 bits; each
+  // factor is held first, so that no product here wraps
+  IE_CHECK(a.tokens >= 0 && a.tokens < (1ll << 24) && a.tokens * a.heads < (1ll << 31) / 128,
+           "%s: %lld query tokens", who, (long long)a.tokens);
   IE_CHECK(a.seqs >= 0 && a.seqs <= a.tokens + (1 << 20) &&
                a.seqs * (int64_t)a.heads < (1ll << 31) / 256,
            "%s: %lld sequences", who, (long long)a.seqs);
@@ -26,7 +27,8 @@ int validate(const ie_attention_args& a, const char* who) {
            (long long)a.seqs);
   IE_CHECK(a.tokens == 0 || a.seqs > 0, "%s: tokens without a sequence", who);
   IE_CHECK(a.block_size > 0, "%s: a block size of %d", who, a.block_size);
-  IE_CHECK(a.table_width >= 0 && a.table_width * (int64_t)a.block_size < (1ll << 31) - (1 << 16),
+  IE_CHECK(a.table_width >= 0 && a.table_width < (1ll << 31) &&
+               a.table_width * a.block_size < (1ll << 31) - (1 << 16),
            "%s: a table of %lld blocks of %d", who, (long long)a.table_width, a.block_size);
   IE_CHECK(a.cache_slots >= 0 && a.cache_slots < (1ll << 31), "%s: %lld cache slots", who,
            (long long)a.cache_slots);

@@ -40,6 +40,21 @@ def test_window_attention(kw):
     assert _lib.last_error().startswith("window_attention")
 
 
+@pytest.mark.parametrize("kw", [
+    dict(tokens=(1 << 62) + 2, seqs=(1 << 62) + 2), dict(tokens=1 << 62, seqs=1 << 62),
+    dict(tokens=(1 << 62) + 2, seqs=2, cu_seqlens_q=4096),
+    dict(table_width=(1 << 60) + 4), dict(table_width=1 << 59, block_size=32),
+    dict(table_width=1 << 33, block_size=(1 << 31) - 1)])
+def test_sizes_whose_products_wrap(kw):
+    a = args(**kw)
+    for entry, name in ((_lib.lib().ie_window_attention, "window_attention"),
+                        (_lib.lib().ie_shared_prefix_attention, "shared_prefix_attention")):
+        assert entry(ctypes.byref(a), None, 0, None) == _lib.IE_ERR_INVALID
+        assert _lib.last_error().startswith(name + ": a table of" if "table_width" in kw else
+                                            f"{name}: {kw['tokens']} query tokens")
+    assert _lib.lib().ie_attention_workspace_size(ctypes.byref(a)) == 0
+
+
 @pytest.mark.parametrize("kw", [dict(window=4), dict(sinks=4), dict(prefix_len=65),
                                 dict(prefix_len=-1), dict(heads=3)])
 def test_shared_prefix_attention(kw):
