@@ -71,18 +71,23 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
   return ((uint64_t)ordered(x) << 32) | (0xFFFFFFFFu - index);
 }
 
-// Sums relative to the maximum m: weights are 2^(x log2 e - scaled(m)).
+// Sums relative to the reference m, the maximum held to [-kFinite, kFinite]: weights are
+// 2^(x log2 e - scaled(m)).  The argument is one FMA, so it is off by the rounding of
+// scaled(m), the same for all of a reference's weights and taken back at the end; within
+// the range that is 1/16 at most.  A finite mask (-1e30, a type's lowest value) then
+// has weight 0 under any reference, and where the row's maximum itself is out of
+// range its sums are computed again from differences (`far_sums`).
 struct Sums {
   float m, s, u;
 };
+constexpr float kFinite = 1048576.0f;
 // __fmul_rn: rounded once everywhere, never contracted into an FMA with a
 // following difference (whose sums would then disagree on the reference)
-__device__ __forceinline__ float scaled(float m) {
-  return m == -INFINITY ? 0.0f : __fmul_rn(m, kLog2e);
-}
-// a's sums taken relative to the larger maximum m
+__device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, kLog2e); }
+__device__ __forceinline__ Sums no_sums() { return {-kFinite, 0.0f, 0.0f}; }
+// a's sums taken relative to the larger reference m
 __device__ __forceinline__ Sums rescaled(Sums a, float m) {
-  const float d = a.m == -INFINITY ? -INFINITY : scaled(a.m) - scaled(m);
+  const float d = scaled(a.m) - scaled(m);
   const float f = ex2(d);
   return {m, a.s * f, f * (a.u + fmaxf(d, kFar) * a.s)};
 }
@@ -104,8 +109,8 @@ __device__ __forceinline__ Sums warp_merge(Sums a) {
 }
 // the same of the first n entries of a shared array, n <= 64, by a whole warp
 __device__ __forceinline__ Sums warp_merge(const Sums* all, int n, int lane) {
-  const Sums none{-INFINITY, 0.0f, 0.0f};
-  return warp_merge(merge(lane < n ? all[lane] : none, lane + 32 < n ? all[lane + 32] : none));
+  return warp_merge(merge(lane < n ? all[lane] : no_sums(),
+                          lane + 32 < n ? all[lane + 32] : no_sums()));
 }
 
 template <typename T> struct Vec {
@@ -244,6 +249,61 @@ struct Row {
   }
 };
 
+// The sums of a row whose maximum lies outside (-kFinite, kFinite), by a whole CTA that
+// reads the row twice: for the maximum, then for weights 2^((x - m) log2 e).  m itself is
+// not finite where the row has +inf or nothing above -inf, and the sums are then NaN.
+template <typename T, int kThreads>
+__device__ __noinline__ Sums far_sums(const Row<T, kThreads>& row, float* shared) {
+  constexpr int kPer = Vec<T>::kPer, kWarps = kThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float m = -INFINITY;
+  for (int64_t v = tid; v < row.nvec; v += kThreads) {
+    float f[kPer];
+    row.load(v, row.nvec, f);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) m = fmaxf(m, f[j]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  __syncthreads();
+  if (lane == 0) shared[warp] = m;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, shared[w]);
+  float s = 0.0f, u = 0.0f;
+  for (int64_t v = tid; v < row.nvec; v += kThreads) {
+    float f[kPer];
+    row.load(v, row.nvec, f);
+    float vs = 0.0f, vu = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int64_t e = row.first(v) + j;
+      if (e < 0 || e >= row.vocab) continue;
+      const float d = (f[j] - m) * kLog2e, w = ex2(d);
+      vs += w;
+      vu = fmaf(w, fmaxf(d, kFar), vu);
+    }
+    s += vs;
+    u += vu;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(~0u, s, o);
+    u += __shfl_xor_sync(~0u, u, o);
+  }
+  __syncthreads();
+  if (lane == 0) {
+    shared[2 * warp] = s;
+    shared[2 * warp + 1] = u;
+  }
+  __syncthreads();
+  s = u = 0.0f;
+  for (int w = 0; w < kWarps; ++w) {
+    s += shared[2 * w];
+    u += shared[2 * w + 1];
+  }
+  return {m, s, u};
+}
+
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads)
 token_logprobs_kernel(const Params p) {
@@ -271,7 +331,7 @@ token_logprobs_kernel(const Params p) {
   const int64_t it0 = iters * rank / ranks, it1 = iters * (rank + 1) / ranks;
   const int64_t end = min(row.nvec, it1 * kThreads * kVecs);
 
-  Sums mine{-INFINITY, 0.0f, 0.0f};
+  Sums mine = no_sums();
   uint32_t tmax = 0;       // ordered; 0 is below every value
   // the given token's logit arrives meanwhile
   int64_t token = -1;
@@ -292,7 +352,7 @@ token_logprobs_kernel(const Params p) {
 #pragma unroll
     for (int i = 1; i < kVecs; ++i) big.add(raw[i]);
     const float bm = big.value();
-    if (bm > mine.m) mine = rescaled(mine, bm);
+    if (bm > mine.m) mine = rescaled(mine, fminf(bm, kFinite));
     const uint64_t ref = f32x2(-scaled(mine.m), -scaled(mine.m));
     const uint64_t log2e = f32x2(kLog2e, kLog2e);
     uint64_t s = 0, u = 0;
@@ -458,10 +518,16 @@ token_logprobs_kernel(const Params p) {
     }
   }
   __syncthreads();
-  const Sums c = warp_merge(all_sums, ranks * kWarps, lane);
+  Sums c = warp_merge(all_sums, ranks * kWarps, lane);
+  // the weights' reference is the rounded product m log2 e, or m itself
+  float off = fmaf(c.m, kLog2e, -scaled(c.m));
+  if (fabsf(c.m) >= kFinite) {        // the same in every thread
+    __syncthreads();                  // all have read all_sums
+    c = far_sums<T, kThreads>(row, reinterpret_cast<float*>(all_sums));
+    off = 0.0f;
+  }
   const float log2s = log2f(c.s);
-  // log sum e^(x - m): the weights' reference is the rounded product m log2 e
-  const float logs = (log2s - fmaf(c.m, kLog2e, -scaled(c.m))) * kLn2;
+  const float logs = (log2s - off) * kLn2;      // log sum e^(x - m)
   if (tid == 0) {
     p.logprobs[r] = token >= 0 && token < p.vocab ? (given - c.m) - logs : -INFINITY;
     p.entropy[r] = (log2s - c.u / c.s) * kLn2;

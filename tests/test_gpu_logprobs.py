@@ -131,6 +131,94 @@ def test_lowest_values_and_large_logits(dtype):
     check(x + 5000.0, t, 8)
 
 
+def check_masked(logits, tokens, top):
+    """As ``check``, with a tolerance that knows nothing of masked logits: with
+    d = x - max, only terms of |d| < 200 reach the sums (e^-200 is below every f32 sum's
+    last bit); their arguments are rounded once (2^-24 |d| log2 e), their exponential is
+    good to 2^-22 and they are summed in several hundred steps; a result beyond that
+    range is a difference of logits, rounded twice."""
+    x = logits.double().cpu().numpy()
+    got = token_logprobs(logits, tokens, top=top)
+    t = tokens.cpu().numpy()
+    for r in range(x.shape[0]):
+        d = x[r] - x[r].max()
+        p = np.exp(d)
+        s = p.sum()
+        logp = d - np.log(s)
+        near = d > -200
+        ent = np.log(s) - (p[near] * d[near]).sum() / s
+        tol = 2.0 ** -23 * (-d[near].min() + 300) + 1e-6
+        bound = tol + 2.0 ** -22 * np.abs(logp)
+
+        def held(value, at):
+            if logp[at] <= -(2.0 ** 128 - 2.0 ** 103):      # rounds to -inf in f32
+                return value == -np.inf
+            return abs(value - logp[at]) <= bound[at]
+
+        assert held(got.logprobs[r].item(), t[r])
+        assert abs(got.entropy[r].item() - ent) <= tol * (1 + ent)
+        order = np.lexsort((np.arange(x.shape[1]), -x[r]))[:top]
+        assert got.top_tokens[r].tolist() == order.tolist()
+        best = got.top_logprobs[r].double().cpu().numpy()
+        assert all(held(b, at) for b, at in zip(best, order))
+
+
+MASKS = [-1e9, -5e9, -1e10, -1e30, "lowest"]
+
+
+def mask_of(value, dtype):
+    low = torch.finfo(dtype).min
+    return low if value == "lowest" else max(value, low)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", MASKS)
+@pytest.mark.parametrize("rows,vocab", [(2, 128256), (3, 5000), (600, 3000)])
+def test_finite_masks_over_whole_runs(dtype, value, rows, vocab):
+    """A mask that leaves a few neighbouring tokens: most threads see masked logits alone."""
+    x, t = make(rows, vocab, dtype, seed=vocab)
+    masked = torch.full_like(x, mask_of(value, dtype))
+    for r, n in zip(range(rows), (1, 700, 40) * rows):
+        at = (r * 997) % (vocab - n)
+        masked[r, at:at + n] = x[r, at:at + n]
+        t[r] = at if r % 2 else t[r]
+    check_masked(masked[:3], t[:3], 20)
+    whole = token_logprobs(masked, t, top=20)
+    for a, b in zip(whole, token_logprobs(masked[-3:], t[-3:], top=20)):
+        torch.testing.assert_close(a[-3:], b, rtol=1e-6, atol=1e-4)
+        assert not torch.isnan(a.float()).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", MASKS)
+@pytest.mark.parametrize("rows,vocab", [(2, 128256), (3, 33), (600, 3000)])
+def test_rows_that_a_finite_mask_covers_whole(dtype, value, rows, vocab):
+    x = torch.full((rows, vocab), mask_of(value, dtype), dtype=dtype, device="cuda")
+    t = torch.arange(rows, device="cuda") % vocab
+    check_masked(x[:3], t[:3], 5)
+    got = token_logprobs(x, t, top=5)
+    torch.testing.assert_close(got.entropy, torch.full_like(got.entropy, np.log(vocab)),
+                               rtol=0, atol=4e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+@pytest.mark.parametrize("size", [2.0 ** 20 - 64, 2.0 ** 20, 2.0 ** 20 + 64, 3e9, 1e30, 3e38])
+def test_maxima_of_any_size(dtype, scale, size):
+    """Logits around a large value of either sign, spread over the type's last bits,
+    beside masked ones."""
+    step = max(abs(torch.finfo(dtype).eps * size), 0.25)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = scale * size + torch.randint(-8, 9, (3, 20000), generator=gen, device="cuda") * step
+    x = x.to(dtype)
+    t = torch.randint(0, 20000, (3,), generator=gen, device="cuda")
+    check_masked(x, t, 8)
+    x[:, 3000:19000] = torch.finfo(dtype).min
+    check_masked(x, t, 8)
+    x[:, :5] = 0.0
+    check_masked(x, t, 8)
+
+
 def test_not_finite():
     x, t = make(5, 3001, torch.float32, seed=5)
     clean = token_logprobs(x, t, top=4)
