@@ -30,6 +30,8 @@
 // bound and a sorted list per CTA: 64 rows 16.2 us, 16 bf16 rows 11.3 against 7.9).
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "f32x2.cuh"
 
@@ -556,9 +558,14 @@ int launch(Params p, cudaStream_t s) {
     ranks *= 2;
   p.batches = (int)((iters + ranks - 1) / ranks + 1);
   const size_t smem = p.top > 0 ? (size_t)p.batches * kThreads * 4 : 0;
+  // what the longest row needs of a full cluster may be above kMaxBatches
+  constexpr int64_t longest =
+      (IE_LOGPROBS_MAX_VOCAB + Vec<T>::kPer - 1 + per_iter - 1) / per_iter;
+  constexpr int64_t most = std::max<int64_t>(kMaxBatches / kThreads,
+                                             (longest + kMaxCluster - 1) / kMaxCluster) + 1;
   auto kernel = token_logprobs_kernel<T, kThreads>;
   static std::atomic<int> allowed[kMaxDevices];
-  if (int rc = allow_smem(kernel, kMaxBatches * 4 + kThreads * 4, allowed)) return rc;
+  if (int rc = allow_smem(kernel, (int)most * kThreads * 4, allowed)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.rows * ranks));
   cfg.blockDim = dim3(kThreads);

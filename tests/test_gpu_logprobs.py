@@ -264,6 +264,15 @@ def test_strides_and_alignments(dtype, shift):
     check(big[::2, shift:shift + 1100], t[:3] % 1100, 6)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [2097152, 2097151, 2097150, 2097149])
+def test_largest_vocabulary(dtype, vocab):
+    x, t = make(2, vocab + 3, dtype, seed=8)
+    for row in (x[:1, :vocab], x[1:, 3:]):      # aligned, and from an odd element on
+        check(row, t[:1] % vocab, 64)
+        check(row, t[:1] % vocab, 0)
+
+
 def test_one_row_for_many_tokens():
     x, t = make(1, 3000, torch.float32, seed=9)
     check(x.expand(5, -1), torch.arange(5, device="cuda") * 500, 3)
