@@ -1055,6 +1055,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
 
       // a sum that is not finite is the row's own: only keys that it sees enter it
       uint32_t again = __ballot_sync(~0u, live && l - l == 0.0f && !(check == 0.0f));
+      if (again) __syncwarp();       // the rows' own stores come before what other lanes write
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;

@@ -128,6 +128,23 @@ def test_values_behind_the_mask_do_not_matter(hd, dtype, bad):
     assert not torch.isfinite(got[at:at + 40]).any()
 
 
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16)])
+@pytest.mark.parametrize("window", [0, 1900])
+def test_values_behind_the_mask_of_split_rows_do_not_matter(hd, dtype, window):
+    """Rows in parts: what is computed again replaces the part's first result."""
+    b = Batch([2000], 4, 1, hd, dtype, 16, query=[300], seed=30)
+    out = torch.empty_like(b.q)
+    assert _lib.lib().ie_attention_workspace_size(ctypes.byref(c_args(b, out, window=window))) > 0
+    want, weight, largest = b.oracle(window=window, sinks=2)
+    for at in (1750, 1999):
+        b.v[int(b.tables[0, at // 16]) * 16 + at % 16] = float("nan")
+    for _ in range(20):
+        got = window_attention(b.q, b.k, b.v, b.tables, b.ctx, 16, window=window, sinks=2,
+                               **b.lens())
+        assert_close(got[:50], want[:50], weight[:50], largest, hd)
+        assert torch.isnan(got[50:]).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_large_scores(dtype):
     """Scores of several hundred: the maximum is subtracted before the exponential,
