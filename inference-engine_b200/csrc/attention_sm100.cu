@@ -42,12 +42,14 @@
 // operands have; scores, sums and outputs are f32.
 //
 // A key that some rows of a tile see and others do not enters the others'
-// product with weight 0; a NaN or infinite V there would still poison them.  Rows
-// that come out not finite although their weights are finite are therefore computed
-// again key by key, leaving out what they do not see.
+// product with weight 0; a NaN or infinite V there would still spoil them.  For a row
+// that comes out not finite although its weights are finite, a warp looks through the
+// keys that the row met but does not see; where it finds such a value, it computes the
+// row's output again over the keys that the row sees.
 //
-// Every wait has a limit; a wait that runs out sets an error bit
-// (ie_kernel_status) and all roles leave.
+// Every wait has a limit, counted from the last sign that rows are being computed again
+// (which takes time in proportion to their contexts); a wait that runs out sets an error
+// bit (ie_kernel_status) and all roles leave.
 #include <cuda.h>
 
 #include <mutex>
@@ -120,23 +122,34 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// False once the limit has passed or another role has given up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* quit) {
+// What the roles tell one another: that one has given up, and (a count that moves) that
+// rows are being computed again, for which the others wait as long as it takes.
+struct Signals {
+  int quit, beat;
+};
+// False once the limit has passed without a beat or another role has given up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile Signals* x) {
   if (mbar_try(bar, parity)) return true;
-  const long long t0 = clock64();
+  long long t0 = clock64();
+  int beat = x->beat;
   while (true) {
     if (mbar_try(bar, parity)) return true;
-    if (*quit) return false;
+    if (x->quit) return false;
     if (clock64() - t0 > kWaitCycles) {
-      atomicOr(&g_attention_status, 1u);
-      *quit = 1;
-      return false;
+      const int now = x->beat;
+      if (now == beat) {
+        atomicOr(&g_attention_status, 1u);
+        x->quit = 1;
+        return false;
+      }
+      beat = now;
+      t0 = clock64();
     }
   }
 }
 // The same for a whole warp: all lanes get one answer.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* quit) {
-  return __all_sync(~0u, mbar_wait(bar, parity, quit));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile Signals* x) {
+  return __all_sync(~0u, mbar_wait(bar, parity, x));
 }
 // True in one lane of a converged warp.  The instructions of the asynchronous units take
 // their operands from uniform registers: a whole warp runs the code around them
@@ -305,7 +318,7 @@ struct Control {
   int slots[2][kTile];                     // cache rows of a key tile
   alignas(16) uint32_t invalid[kInvalidRing][4];   // keys of a tile whose page is not there
   uint32_t tmem;
-  int quit;
+  Signals signals;
 };
 static_assert(sizeof(Control) <= 2048, "control block");
 
@@ -343,7 +356,7 @@ struct Items {
   __device__ __forceinline__ explicit Items(int first) : item(first) {}
   // -1: no more (or another role gave up)
   __device__ __forceinline__ void next(Control* c) {
-    if (!warp_wait(smem_u32(&c->next_full), phase, &c->quit)) {
+    if (!warp_wait(smem_u32(&c->next_full), phase, &c->signals)) {
       item = -1;
       return;
     }
@@ -357,7 +370,7 @@ struct Items {
 // The asking, by one of the readers, once all have read the answer before (`n` asked
 // so far).  A refusal ends the reader's loop: nobody asks again.
 __device__ __forceinline__ void ask_next(Control* c, uint32_t n) {
-  if (n > 0 && !warp_wait(smem_u32(&c->next_empty), (n - 1) & 1, &c->quit)) return;
+  if (n > 0 && !warp_wait(smem_u32(&c->next_empty), (n - 1) & 1, &c->signals)) return;
   if (elect()) {
     mbar_expect(smem_u32(&c->next_full), 16);
     try_take(smem_u32(c->next), smem_u32(&c->next_full));
@@ -431,52 +444,127 @@ __device__ __forceinline__ void locate(const TileParams& a, Work& w, int tile) {
   w.j1 = (int)((int64_t)tiles * (w.part + 1) / a.parts);
 }
 
-// ---- a row computed key by key (see the top) ------------------------------------------
-// Warp-wide: o, m, l of the row of query token t, head h at position pos over the
-// key tiles of the work item (twin: of its stream `stream`).
+// ---- rows that a value behind their mask has spoilt (see the top) ------------------------
+// The virtual keys v that a row sees: v <= vmax and (v >= vmin or v < sinks).
+struct Seen {
+  int vmax, vmin;
+  __device__ __forceinline__ Seen(const Params& p, const Work& w, int pos) {
+    const int shift = w.lo - w.ns;
+    vmax = pos < 0 ? -1 : min(pos - shift, w.n - 1);
+    vmin = max(p.window > 0 ? pos - p.window + 1 : 0, p.key_start) - shift;
+  }
+  __device__ __forceinline__ bool one(const Params& p, int v) const {
+    return v <= vmax && (v >= vmin || v < p.sinks);
+  }
+  __device__ __forceinline__ bool tile(const Params& p, int v0) const {     // all of its keys
+    return v0 + kTile - 1 <= vmax && (v0 >= vmin || v0 + kTile <= p.sinks);
+  }
+};
+// Calls f(v, seen) for this lane's keys of the row's tiles, 32 at a time, where there is
+// work: all of them, or (unseen) only in tiles that the row does not see whole.  Ends
+// when f returns true, which it does in all lanes or none.
+template <typename F>
+__device__ __forceinline__ bool keys_of_row(const TileParams& a, const Work& w, Control* c,
+                                            const Seen& see, int stream, bool unseen, F f) {
+  const int lane = threadIdx.x & 31;
+  for (int j = w.j0; j < w.j1; ++j) {
+    if (a.twin && ((j - w.j0) & 1) != stream) continue;
+    const int v0 = j * kTile;
+    if (unseen && see.tile(a.p, v0)) continue;
+    for (int i = 0; i < kTile && v0 + i < w.n; i += 32) {
+      if (lane == 0) atomicAdd(&c->signals.beat, 1);
+      const int v = v0 + i + lane;
+      if (f(v, see.one(a.p, v))) return true;
+    }
+  }
+  return false;
+}
+__device__ __forceinline__ int slot_of_virtual(const TileParams& a, const Work& w, int v) {
+  const Params& p = a.p;
+  const int32_t* table = p.tables + (a.mode == kPrefix ? 0 : (int64_t)w.seg * p.table_stride);
+  return v < w.n ? cache_slot(p, table, v < w.ns ? v : w.lo + v - w.ns) : -1;
+}
+
+// Warp-wide: whether a key that the row at `pos` does not see, but its products met, has
+// a value that is not finite.  A lane looks through one key's row.
 template <typename T, int HD>
-__device__ __noinline__ void row_again(const TileParams& a, const Work& w, int t, int h, int pos,
-                                       int stream, float* m_out, float* l_out,
+__device__ __noinline__ bool spoilt(const TileParams& a, const Work& w, Control* c, int pos,
+                                    int stream) {
+  const Params& p = a.p;
+  const T* vc = static_cast<const T*>(p.v) + w.kvh * p.head_stride;
+  constexpr uint32_t kExp = dtype_of<T>() == IE_DT_BF16 ? 0x7F80u : 0x7C00u;
+  return keys_of_row(a, w, c, Seen(p, w, pos), stream, true, [&](int v, bool seen) {
+    const int slot = seen ? -1 : slot_of_virtual(a, w, v);
+    bool bad = false;
+    if (slot >= 0) {
+      const uint4* row = reinterpret_cast<const uint4*>(vc + slot * p.slot_stride);
+#pragma unroll
+      for (int k = 0; k < HD / 8; ++k) {
+        const uint4 x = __ldg(row + k);
+        for (uint32_t y : {x.x, x.y, x.z, x.w})
+          bad = bad || (y & kExp) == kExp || (y >> 16 & kExp) == kExp;
+      }
+    }
+    return __any_sync(~0u, bad) != 0;
+  });
+}
+
+// Warp-wide: o, relative to the 2^m that the row's sums have, of query token t, head h,
+// over the keys that it sees.  A lane computes one key's score; lane + 32 e is an element
+// of o.  Ends early when every element is NaN, which it then stays.
+template <typename T, int HD>
+__device__ __noinline__ void row_again(const TileParams& a, const Work& w, Control* c, int t,
+                                       int h, int pos, int stream, float m,
                                        float (&o)[HD / 32]) {
   const Params& p = a.p;
   const int lane = threadIdx.x & 31;
-  const int32_t* table = p.tables + (a.mode == kPrefix ? 0 : (int64_t)w.seg * p.table_stride);
-  const T* q = static_cast<const T*>(p.q) + t * p.q_token + h * p.q_head;
+  const uint4* q =
+      reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + t * p.q_token + h * p.q_head);
   const T* kc = static_cast<const T*>(p.k) + w.kvh * p.head_stride;
-  const T* vc = static_cast<const T*>(p.v) + w.kvh * p.head_stride;
-  float qv[HD / 32];
+  const T* vc = static_cast<const T*>(p.v) + w.kvh * p.head_stride + lane;
 #pragma unroll
-  for (int e = 0; e < HD / 32; ++e) {
-    qv[e] = to_f32<T>(q[lane + 32 * e]) * p.scale2;
-    o[e] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int j = w.j0; j < w.j1; ++j) {
-    if (a.twin && ((j - w.j0) & 1) != stream) continue;
-    for (int v = j * kTile; v < min((j + 1) * kTile, w.n); ++v) {
-      const int key = v < w.ns ? v : w.lo + v - w.ns;
-      if (key > pos || key < p.key_start ||
-          !(p.window == 0 || key > pos - p.window || key < p.sinks))
-        continue;
-      const int slot = cache_slot(p, table, key);
-      if (slot < 0) continue;
-      const int64_t at = slot * p.slot_stride + lane;
+  for (int e = 0; e < HD / 32; ++e) o[e] = 0.0f;
+  keys_of_row(a, w, c, Seen(p, w, pos), stream, false, [&](int v, bool seen) {
+    const int slot = seen ? slot_of_virtual(a, w, v) : -1;
+    if (!__any_sync(~0u, slot >= 0)) return false;
+    float weight = 0.0f;
+    if (slot >= 0) {
+      const uint4* k = reinterpret_cast<const uint4*>(kc + slot * p.slot_stride);
       float s = 0.0f;
 #pragma unroll
-      for (int e = 0; e < HD / 32; ++e) s = fmaf(qv[e], to_f32<T>(kc[at + 32 * e]), s);
+      for (int i = 0; i < HD / 8; ++i) {
+        const uint4 x = __ldg(q + i), y = __ldg(k + i);
+        const T* xs = reinterpret_cast<const T*>(&x);
+        const T* ys = reinterpret_cast<const T*>(&y);
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(~0u, s, off);
-      const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
-      const float f = ex2(m - ref), wgt = ex2(s - ref);
-      m = mn;
-      l = fmaf(l, f, wgt);
-#pragma unroll
-      for (int e = 0; e < HD / 32; ++e)
-        o[e] = fmaf(wgt, to_f32<T>(vc[at + 32 * e]), o[e] * f);
+        for (int e = 0; e < 8; ++e) s = fmaf(to_f32<T>(xs[e]), to_f32<T>(ys[e]), s);
+      }
+      weight = ex2(fmaf(s, p.scale2, -m));
     }
-  }
-  *m_out = m;
-  *l_out = l;
+    constexpr int kAtOnce = 8;      // keys whose values are in flight
+#pragma unroll 1
+    for (int i = 0; i < 32; i += kAtOnce) {
+      float value[kAtOnce][HD / 32];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int at = max(__shfl_sync(~0u, slot, i + u), 0);
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e)
+          value[u][e] = to_f32<T>(vc[at * p.slot_stride + 32 * e]);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const float x = __shfl_sync(~0u, weight, i + u);
+        const bool there = __shfl_sync(~0u, slot, i + u) >= 0;
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) o[e] = there ? fmaf(x, value[u][e], o[e]) : o[e];
+      }
+    }
+    bool over = true;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) over = over && o[e] != o[e];
+    return __all_sync(~0u, over) != 0;
+  });
 }
 
 // 32 bytes of a thread's own row: a whole sector a store where the row allows it
@@ -544,7 +632,7 @@ __device__ void gather_role(const TileParams& a, uint8_t* base, Control* c) {
     const uint32_t parity = (item / L::kStages - 1) & 1;
     if (mbar_try(bar, parity)) return true;
     flush();                 // what waits for us must not wait for ever
-    return mbar_wait(bar, parity, &c->quit);
+    return mbar_wait(bar, parity, &c->signals);
   };
   auto commit = [&]() {
     cp_commit();
@@ -655,7 +743,7 @@ __device__ void tma_role(const TileParams& a, const CUtensorMap* maps, uint8_t* 
         const int at = rows > 0 ? row : outside;
         const uint32_t st = item % L::kStages, bar = smem_u32(&c->full[st]);
         if (item >= L::kStages &&
-            !warp_wait(smem_u32(&c->empty[st]), (item / L::kStages - 1) & 1, &c->quit)) {
+            !warp_wait(smem_u32(&c->empty[st]), (item / L::kStages - 1) & 1, &c->signals)) {
           // what has been started ends before the CTA does
           const long long t0 = clock64();
           constexpr uint32_t kBack = L::kStages & ~1;
@@ -728,7 +816,7 @@ __device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t*
     for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
       if (w.j0 >= w.j1) continue;
-      if (n > 0 && !warp_wait(smem_u32(&c->q_free), (n - 1) & 1, &c->quit)) break;
+      if (n > 0 && !warp_wait(smem_u32(&c->q_free), (n - 1) & 1, &c->signals)) break;
       ++n;
       const int tiles = row_tiles_of(a, w);
       if (kTma) {
@@ -761,12 +849,12 @@ __device__ void query_role(const TileParams& a, const CUtensorMap* map, uint8_t*
     }
   } while (next_item(it));
   // a load that nothing waited for (the others gave up) ends before the CTA does
-  if (kTma && c->quit && n > 0) {
+  if (kTma && c->signals.quit && n > 0) {
     const long long t0 = clock64();
     while (!mbar_try(bar, (n - 1) & 1) && clock64() - t0 < kWaitCycles) {
     }
   }
-  if (c->quit && asks && asked > 0) {      // nor does an answer come after it
+  if (c->signals.quit && asks && asked > 0) {      // nor does an answer come after it
     const long long t0 = clock64();
     while (!mbar_try(smem_u32(&c->next_full), (asked - 1) & 1) && clock64() - t0 < kWaitCycles) {
     }
@@ -799,10 +887,10 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c,
       }
     }
   } cur;
-  auto full = [&](const Cursor& x) { return warp_wait(full0 + 8 * x.stage, x.phase, &c->quit); };
+  auto full = [&](const Cursor& x) { return warp_wait(full0 + 8 * x.stage, x.phase, &c->signals); };
   auto release = [&](const Cursor& x) { tc_commit(leader, empty0 + 8 * x.stage); };
   auto p_ready = [&](int s, int half) {
-    return warp_wait(p_ready0 + 16 * s + 8 * half, np >> s & 1, &c->quit);
+    return warp_wait(p_ready0 + 16 * s + 8 * half, np >> s & 1, &c->signals);
   };
   auto scores = [&](int s, int q, const Cursor& x) {      // S_s = Q_q K^T
     const uint32_t ql = q_lo + q * kStep, kl = k_lo + x.stage * kStep, d = tmem + s * kTile;
@@ -837,7 +925,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c,
       locate(a, w, tile);
       const int nt = w.j1 - w.j0;
       if (nt <= 0) continue;
-      if (!warp_wait(smem_u32(&c->q_full), nq, &c->quit)) return;
+      if (!warp_wait(smem_u32(&c->q_full), nq, &c->signals)) return;
       nq ^= 1;
       if (a.twin) {
         Cursor v[2];        // V tile of each stream's last scores
@@ -920,15 +1008,13 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
       int pos = -1;
       if (live) pos = a.mode == kPrefix ? position_of(p, sequence_of(p, t), t)
                                         : w.ctx - w.ntok + tok;
-      // virtual key v is seen iff v <= vmax and (v >= vmin or v < sinks)
-      const int shift = w.lo - w.ns;
-      const int vmax = pos < 0 ? -1 : min(pos - shift, w.n - 1);
-      const int vmin = max(p.window > 0 ? pos - p.window + 1 : 0, p.key_start) - shift;
+      const Seen seen(p, w, pos);
+      const int vmax = seen.vmax, vmin = seen.vmin;
 
       float m = -INFINITY, l = 0.0f;
       int done = 0;
       for (int j = w.j0 + (a.twin ? s : 0); j < w.j1; j += a.twin ? 2 : 1) {
-        if (!warp_wait(smem_u32(&c->s_full[s]), n_s & 1, &c->quit)) return;
+        if (!warp_wait(smem_u32(&c->s_full[s]), n_s & 1, &c->signals)) return;
         ++n_s;
         tc_fence_after();
         uint32_t raw[kTile];
@@ -937,8 +1023,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
         const int v0 = j * kTile;
         const uint4 bad = *reinterpret_cast<const uint4*>(
             c->invalid[(tile0 + (j - w.j0)) % kInvalidRing]);
-        const bool whole = v0 + kTile - 1 <= vmax && (v0 >= vmin || v0 + kTile <= p.sinks) &&
-                           (bad.x | bad.y | bad.z | bad.w) == 0;
+        const bool whole = seen.tile(p, v0) && (bad.x | bad.y | bad.z | bad.w) == 0;
         if (!__all_sync(~0u, whole)) {
           const uint32_t words[4] = {bad.x, bad.y, bad.z, bad.w};
 #pragma unroll
@@ -1014,7 +1099,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
       T* out = static_cast<T*>(p.out) + (int64_t)t * p.out_token + (int64_t)head * HD;
       float inv = 0.0f, check = 0.0f;
       if (done > 0) {
-        if (!warp_wait(smem_u32(&c->o_done[s]), n_o & 1, &c->quit)) return;
+        if (!warp_wait(smem_u32(&c->o_done[s]), n_o & 1, &c->signals)) return;
         ++n_o;
         tc_fence_after();
         inv = l == 0.0f ? 0.0f : (p.slots ? 1.0f : 1.0f / l);
@@ -1061,18 +1146,18 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
         again &= again - 1;
         const int tt = __shfl_sync(~0u, t, src), hh = __shfl_sync(~0u, head, src);
         const int pp = __shfl_sync(~0u, pos, src);
-        float o[HD / 32], m2, l2;
-        row_again<T, HD>(a, w, tt, hh, pp, s, &m2, &l2, o);
+        const float mm = __shfl_sync(~0u, m, src), ll = __shfl_sync(~0u, l, src);
+        if (!spoilt<T, HD>(a, w, c, pp, s)) continue;     // what it sees is not finite
+        float o[HD / 32];
+        row_again<T, HD>(a, w, c, tt, hh, pp, s, mm, o);
         const int64_t at2 = ((int64_t)tt * p.heads + hh) * p.slots + slot;
-        const float i2 = l2 == 0.0f ? 0.0f : 1.0f / l2;
 #pragma unroll
         for (int e = 0; e < HD / 32; ++e) {
           if (p.slots) p.part_o[at2 * HD + lane + 32 * e] = o[e];
           else
             static_cast<T*>(p.out)[(int64_t)tt * p.out_token + (int64_t)hh * HD + lane + 32 * e] =
-                from_f32<T>(o[e] * i2);
+                from_f32<T>(o[e] / ll);
         }
-        if (p.slots && lane == 0) p.part_ml[at2] = make_float2(m2, l2);
       }
     }
   }
@@ -1103,7 +1188,7 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
     mbar_init(smem_u32(&c->q_free), 1);
     mbar_init(smem_u32(&c->next_full), 1);
     mbar_init(smem_u32(&c->next_empty), W::kReaders);
-    c->quit = 0;
+    c->signals = Signals{0, 0};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == W::kIssue) {
@@ -1141,7 +1226,7 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (c->quit) {
+  if (c->signals.quit) {
     if (warp == W::kIssue && (threadIdx.x & 31) == 0) {
       mbar_init(smem_u32(&c->slots[0][0]), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

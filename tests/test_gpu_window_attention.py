@@ -145,6 +145,48 @@ def test_values_behind_the_mask_of_split_rows_do_not_matter(hd, dtype, window):
         assert torch.isnan(got[50:]).all()
 
 
+@pytest.mark.parametrize("context,at,bad", [
+    (400000, 100, float("nan")), (400000, 100, float("inf")), (400000, -300, float("nan")),
+    (400000, -300, float("inf")), (1500000, -300, float("nan"))])
+def test_a_broken_value_in_a_long_context(context, at, bad):
+    """1024 queries over a long context (pages in turn), all in one CTA: a value that is
+    not finite reaches the queries that see it, and the others are right, however long it
+    takes to tell them apart (in the longest case more than the limit of a wait)."""
+    block, hd, n = 256, 64, 1024
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda").to(BF16)
+    k, v, q = rnd(9 * block, 1, hd), rnd(9 * block, 1, hd), rnd(n, 1, hd)
+    at %= context
+    table = torch.arange(-(-context // block), device="cuda", dtype=torch.int32) % 8
+    table[at // block] = 8                   # a page of its own
+    slot = table.long()[torch.arange(context, device="cuda") // block] * block \
+        + torch.arange(context, device="cuda") % block
+    rows = torch.arange(3, n, 50, device="cuda")
+    score = q[rows, 0].double() @ k[slot, 0].double().T * hd ** -0.5
+    score.masked_fill_(torch.arange(context, device="cuda")[None]
+                       > (context - n + rows)[:, None], -float("inf"))
+    p = torch.softmax(score, -1)
+    want, weight = (p @ x[slot, 0].double() for x in (v, v.abs()))
+    blind = (context - n + rows < at).cpu().numpy()
+    v[8 * block + at % block] = bad
+    ctx = torch.tensor([context], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 77.0)
+    window_attention(q, k, v, table[None], ctx, block, cu_seqlens_q=cu, max_query_len=256,
+                     max_context_len=128, out=out)
+    status = ctypes.c_uint32()
+    _lib.check(_lib.lib().ie_kernel_status(ctypes.byref(status), 1))
+    assert status.value == 0
+    assert blind.any() == (at != 100)
+    if blind.any():
+        # |q|_1 |k|_inf bounds a score's rounding as in the oracle
+        largest = float((q[rows, 0].double().abs() @ k[slot, 0].double().abs().T).max()) / hd ** 0.5
+        assert_close(out[rows, 0][blind], want.cpu().numpy()[blind], weight.cpu().numpy()[blind],
+                     largest, hd)
+    sees = out[context - n + torch.arange(n) >= at] if at != 100 else out
+    assert not torch.isfinite(sees).any()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_large_scores(dtype):
     """Scores of several hundred: the maximum is subtracted before the exponential,
