@@ -266,7 +266,8 @@ int ie_rope_kv(const void* qkv, int64_t ld_qkv, int32_t dtype, int64_t tokens, i
  * same for every sequence and are looked up in the FIRST row of block_tables;
  * they are read once for the whole batch (a short prefix once a sequence, from L2).
  *
- * Both: a query that sees nothing (an empty context) gets zeros.  A key whose
+ * Both: a query that sees nothing (an empty context, or a token in front of
+ * cu_seqlens_q[0] or from cu_seqlens_q[seqs] on, which is no sequence's) gets zeros.  A key whose
  * table entry names no page of the cache (-1, as a page given back reads) is not
  * seen; K and V rows that are not seen may hold anything, NaN included.
  * Softmax, sums and the join of parts are f32.  f32 rows, head sizes other than

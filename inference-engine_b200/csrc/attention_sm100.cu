@@ -385,6 +385,7 @@ __device__ __forceinline__ void ask_next(Control* c, uint32_t n) {
 struct Work {
   int seg, kvh, part, first;
   int tok0, ctx, ntok;                 // of the segment: first token, context, tokens
+  int begin, end;                      // its sequence's own tokens (see `segment`)
   int lo, ns, n;                       // virtual keys: ns sinks, then from lo
   int j0, j1;
 };
@@ -407,15 +408,18 @@ __device__ __forceinline__ bool segment(const TileParams& a, int item, Work& w, 
   w.part = item % a.parts;
   tile = a.row_tiles - 1 - item / a.parts;      // the longest contexts first
   if (a.mode == kPrefix) {
-    w.tok0 = 0;
-    w.ntok = p.tokens;
+    w.tok0 = w.begin = 0;
+    w.ntok = w.end = p.tokens;
     w.ctx = 0;
   } else {
-    w.tok0 = p.cu_q ? __ldg(p.cu_q + w.seg) : w.seg;
-    w.ntok = p.cu_q ? __ldg(p.cu_q + w.seg + 1) - w.tok0 : 1;
-    // a table of lengths that does not describe [0, tokens) reads and writes nothing
-    if (w.tok0 < 0 || w.tok0 > p.tokens) w.ntok = 0;
-    w.ntok = min(w.ntok, p.tokens - w.tok0);
+    w.begin = p.cu_q ? __ldg(p.cu_q + w.seg) : w.seg;
+    w.end = p.cu_q ? __ldg(p.cu_q + w.seg + 1) : w.seg + 1;
+    // the first and the last segment take in the tokens that are no sequence's, whose rows
+    // see nothing and are zeros
+    w.tok0 = w.seg == 0 ? 0 : w.begin;
+    w.ntok = (w.seg == a.segs - 1 ? p.tokens : min(w.end, p.tokens)) - w.tok0;
+    // a table of lengths that does not begin in [0, tokens] reads and writes nothing
+    if (w.begin < 0 || w.begin > p.tokens) w.ntok = 0;
     w.ctx = context_of(p, w.seg);
   }
   return w.ntok > tile * tokens_of_work(a);
@@ -427,8 +431,11 @@ __device__ __forceinline__ void locate(const TileParams& a, Work& w, int tile) {
     w.lo = w.ns = 0;
     w.n = p.key_end;
   } else {
-    const int first = max(w.ctx - w.ntok + w.first, 0);
-    const int last = w.ctx - w.ntok + min(w.first + tokens_of_work(a), w.ntok) - 1;
+    // the sequence's tokens among the tile's
+    const int t0 = max(w.tok0 + w.first, w.begin);
+    const int t1 = min(w.tok0 + min(w.first + tokens_of_work(a), w.ntok), w.end) - 1;
+    const int first = max(w.ctx - (w.end - t0), 0);
+    const int last = t0 > t1 ? -1 : w.ctx - (w.end - t1);
     w.lo = p.key_start;
     if (p.window > 0) w.lo = max(w.lo, first - p.window + 1);
     w.ns = p.key_start == 0 ? min(p.sinks, w.lo) : 0;
@@ -1007,7 +1014,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
       const int head = w.kvh * p.group + row_head;
       int pos = -1;
       if (live) pos = a.mode == kPrefix ? position_of(p, sequence_of(p, t), t)
-                                        : w.ctx - w.ntok + tok;
+                                        : t >= w.begin && t < w.end ? w.ctx - (w.end - t) : -1;
       const Seen seen(p, w, pos);
       const int vmax = seen.vmax, vmin = seen.vmin;
 

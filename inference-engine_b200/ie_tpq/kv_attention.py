@@ -8,7 +8,8 @@ output and workspace from torch's allocator on the stream they run on, never
 synchronise, and can be captured in a CUDA graph.  Queries are ragged: sequence
 ``s`` owns the tokens ``cu_seqlens_q[s] : cu_seqlens_q[s + 1]`` and its last one
 is at position ``context_lens[s] - 1``; without ``cu_seqlens_q`` every sequence
-has one token (decode).  A query that sees nothing gets zeros.
+has one token (decode).  A query that sees nothing gets zeros, and so does a token
+that ``cu_seqlens_q`` gives to no sequence (the end of a padded batch).
 """
 from __future__ import annotations
 

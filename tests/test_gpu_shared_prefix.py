@@ -83,6 +83,21 @@ def test_several_queries(hd, dtype):
     check(Batch([100 + n for n in query], 8, 2, hd, dtype, 16, query=query, prefix=96, seed=hd))
 
 
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16), (64, F32)])
+@pytest.mark.parametrize("lead,tail", [(0, 2), (0, 200), (5, 0), (140, 3)])
+def test_tokens_of_no_sequence_are_zeros(hd, dtype, lead, tail):
+    query = [7, 40, 3]
+    b = Batch([1300, 1240, 1203], 8, 2, hd, dtype, 16, query=query, prefix=1200, seed=hd)
+    want, weight, largest = b.oracle(prefix=1200)
+    q = torch.randn((lead + 50 + tail, 8, hd), device="cuda").to(dtype)
+    q[lead:lead + 50] = b.q
+    out = torch.full_like(q, float("nan"))
+    shared_prefix_attention(q, b.k, b.v, b.tables, b.ctx, 1200, 16, out=out,
+                            cu_seqlens_q=b.cu + lead, max_query_len=40, max_context_len=1300)
+    assert_close(out[lead:lead + 50], want, weight, largest, hd)
+    assert torch.count_nonzero(out[:lead]) == 0 and torch.count_nonzero(out[lead + 50:]) == 0
+
+
 def test_sequences_shorter_than_the_prefix():
     b = Batch([100, 20, 1, 0, 64], 8, 2, 64, BF16, 16, prefix=64, seed=3)
     got = check(b)

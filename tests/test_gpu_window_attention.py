@@ -295,6 +295,27 @@ def test_graph_capture_follows_the_lengths(query):
     assert_close(out, want, weight, largest, 128)
 
 
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, F16), (64, F32)])
+@pytest.mark.parametrize("context,query", [([500, 300], [40, 9]), ([2000, 64], [5, 3]),
+                                           ([70, 0], [70, 0])])
+@pytest.mark.parametrize("lead,tail", [(0, 1), (0, 300), (3, 0), (150, 5)])
+@pytest.mark.parametrize("lens", [True, False])
+def test_tokens_of_no_sequence_are_zeros(hd, dtype, context, query, lead, tail, lens):
+    """A batch of a fixed number of tokens of which the lengths cover a part, whole or in
+    parts."""
+    b = Batch(context, 4, 2, hd, dtype, 16, query=query, seed=33)
+    want, weight, largest = b.oracle(window=400, sinks=2)
+    n = sum(query)
+    q = torch.randn((lead + n + tail, 4, hd), device="cuda").to(dtype)
+    q[lead:lead + n] = b.q
+    out = torch.full_like(q, float("nan"))
+    window_attention(q, b.k, b.v, b.tables, b.ctx, 16, window=400, sinks=2, out=out,
+                     cu_seqlens_q=b.cu + lead, max_query_len=max(query) if lens else 0,
+                     max_context_len=max(context) if lens else 0)
+    assert_close(out[lead:lead + n], want, weight, largest, hd)
+    assert torch.count_nonzero(out[:lead]) == 0 and torch.count_nonzero(out[lead + n:]) == 0
+
+
 def test_empty_batches():
     b = Batch([5], 4, 2, 64, BF16, 16, seed=15)
     none = torch.empty((0,), dtype=torch.int32, device="cuda")
