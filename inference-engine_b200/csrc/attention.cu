@@ -76,8 +76,9 @@ Params base_params(const ie_attention_args& a) {
   p.cache_rows = (int)a.cache_slots;
   p.block = FastDiv((uint32_t)a.block_size);
   p.group_div = FastDiv((uint32_t)p.group);
-  const int64_t most = 1 << 30;
-  p.window = (int)std::min(a.window, most);
+  // a window of all that a table can address hides nothing
+  const int64_t most = a.table_width * a.block_size;
+  p.window = a.window < most ? (int)a.window : 0;
   p.sinks = (int)std::min(a.sinks, most);
   p.key_end = 0x7FFFFFFF;
   p.scale2 = a.scale * kLog2e;

@@ -81,13 +81,13 @@ __device__ __forceinline__ int context_of(const Params& p, int s) {
   return c < 0 ? 0 : (c < most ? c : (int)most);
 }
 
-// Position of query token t of sequence s; negative: it sees nothing (a token in front of
-// the first sequence or behind the last is no sequence's).
+// Position of query token t of sequence s; -1: it sees nothing (a token in front of the
+// first sequence or behind the last is no sequence's).
 __device__ __forceinline__ int position_of(const Params& p, int s, int t) {
   const int ctx = context_of(p, s);
   if (!p.cu_q) return ctx - 1;
   const int end = __ldg(p.cu_q + s + 1);
-  return t >= __ldg(p.cu_q + s) && t < end ? ctx - (end - t) : -1;
+  return t >= __ldg(p.cu_q + s) && t < end ? max(ctx - (end - t), -1) : -1;
 }
 
 // The keys that a query at `pos` sees within [key_start, key_end), numbered

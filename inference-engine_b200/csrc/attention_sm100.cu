@@ -1014,7 +1014,9 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
       const int head = w.kvh * p.group + row_head;
       int pos = -1;
       if (live) pos = a.mode == kPrefix ? position_of(p, sequence_of(p, t), t)
-                                        : t >= w.begin && t < w.end ? w.ctx - (w.end - t) : -1;
+                                        : t >= w.begin && t < w.end
+                                              ? max(w.ctx - (w.end - t), -1)
+                                              : -1;
       const Seen seen(p, w, pos);
       const int vmax = seen.vmax, vmin = seen.vmin;
 

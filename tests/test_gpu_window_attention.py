@@ -264,6 +264,39 @@ def test_cache_beyond_32_bit_offsets():
         assert_close(got, want, weight, largest, hd)
 
 
+@pytest.mark.parametrize("several", [False, True])
+def test_windows_and_sinks_beyond_2_to_the_30(several):
+    """A context of 2^30 + 2^17 keys (three pages in turn) in which one key outweighs all
+    others: it is seen or not by one position more or less of the window or the sinks."""
+    block, hd = 1 << 16, 64
+    context = (1 << 30) + (1 << 17)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn((3 * block, 1, hd), generator=gen, device="cuda").to(BF16)
+    v = torch.randn((3 * block, 1, hd), generator=gen, device="cuda").to(BF16)
+    q = torch.randn((1, 1, hd), generator=gen, device="cuda").to(BF16)
+    big = q[0, 0].double() * (60 * hd ** 0.5 / q.double().square().sum())
+    k[block + 3, 0] = big.to(BF16)               # a score of 60 against N(0, 1)
+    k[2 * block + 5, 0] = big.to(BF16)
+    ctx = torch.tensor([context], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda") if several else None
+    table = torch.zeros((1, context // block), dtype=torch.int32, device="cuda")
+
+    def sees(slot, **kw):
+        got = window_attention(q, k, v, table, ctx, block, cu_seqlens_q=cu, max_query_len=1,
+                               max_context_len=context, **kw)
+        # 2^31 keys of e^6 at most against e^59: below bf16's last bit
+        return bool((got[0, 0] - v[slot, 0]).abs().max() <= 2.0 ** -7 * v[slot].abs().max())
+
+    table[0, 0] = 1                              # the key at position 3
+    assert sees(block + 3) and sees(block + 3, window=context)
+    assert sees(block + 3, window=context - 3) and not sees(block + 3, window=context - 4)
+    table[0, 0], table[0, 1 << 14] = 0, 2        # the key at position 2^30 + 5
+    at = (1 << 30) + 5
+    assert sees(2 * block + 5, window=10, sinks=at + 1)
+    assert not sees(2 * block + 5, window=10, sinks=at)
+    assert sees(2 * block + 5, window=10, sinks=1 << 40)
+
+
 def test_same_bits_twice_and_on_another_stream():
     b = Batch([700, 3000], 8, 2, 128, BF16, 16, seed=13)
     a = check(b, window=1000, sinks=4)
