@@ -200,7 +200,9 @@ Plan make_plan(const ie_attention_args& a) {
   const int64_t group = a.heads / a.kv_heads;
   int64_t keys = a.table_width * a.block_size;      // of the longest context
   if (a.max_context_len > 0) keys = std::min(keys, a.max_context_len);
-  const int64_t seen = a.window > 0 ? std::min(keys, a.window + a.sinks) : keys;
+  // (held to the keys before they are added)
+  const int64_t reach = std::min(a.window, keys) + std::min(a.sinks, keys);
+  const int64_t seen = a.window > 0 ? std::min(keys, reach) : keys;
   const int64_t per_tile = 128 / group;     // tokens of a row tile of the tensor cores
   // (a group of more than 128 heads has only the decode kernel)
   if (!tensor_cores(a) || (per_tile == 0 && (a.cu_seqlens_q || a.prefix_len > 0))) {
@@ -229,7 +231,7 @@ Plan make_plan(const ie_attention_args& a) {
     // Eight warps an SM, as one CTA or two.  Rows that a window makes equally long also
     // fill one round of four (64 sequences, window 4096: 151 us against 157; uneven
     // ones lose: 32 sequences of up to 32768 448 against 356).
-    const bool even = a.window > 0 && a.window + a.sinks < keys;
+    const bool even = a.window > 0 && reach < keys;
     plan.decode_warps = eight_warps(ctas, plan.slots ? 1 : plan.decode_parts) ? 8
                         : even && plan.decode_parts == 1 && ctas > 2 * kSms && ctas <= 4 * kSms
                             ? 2

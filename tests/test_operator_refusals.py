@@ -76,6 +76,20 @@ def test_workspace_that_is_missing_or_small():
     assert lib.ie_window_attention(None, None, 0, None) == _lib.IE_ERR_INVALID
 
 
+@pytest.mark.parametrize("cu", [None, 4096])
+@pytest.mark.parametrize("dtype", [_lib.IE_DT_BF16, _lib.IE_DT_F32])
+def test_a_window_without_limit_is_planned_like_none(cu, dtype):
+    lib = _lib.lib()
+    one = dict(tokens=1, seqs=1, heads=2, kv_heads=1, table_width=4096, table_stride=4096,
+               cu_seqlens_q=cu, dtype=dtype)
+    want = lib.ie_attention_workspace_size(ctypes.byref(args(**one)))
+    assert want > 0
+    for window, sinks in ((2 ** 63 - 1, 4), (2 ** 63 - 1, 2 ** 63 - 1), (1, 2 ** 63 - 1),
+                          (65536, 0), (65535, 1)):
+        a = args(window=window, sinks=sinks, **one)
+        assert lib.ie_attention_workspace_size(ctypes.byref(a)) == want
+
+
 @pytest.mark.parametrize("head_dim", [1, 33, 255])
 def test_odd_head_sizes_leave_room_for_aligned_pairs(head_dim):
     """The parts' (m, l) pairs follow an odd number of f32 sums on an 8-byte boundary."""
