@@ -26,6 +26,20 @@ class OutOfPages(RuntimeError):
     """The pool has fewer free pages than the call needs; nothing was changed."""
 
 
+def _page_numbers(name: str, pages) -> np.ndarray:
+    """A list or array of page numbers as int32; what int32 cannot hold as it is (floats,
+    numbers beyond its range) is refused, not cast."""
+    a = np.asarray(pages)
+    if a.size == 0:
+        return np.zeros(a.shape, dtype=np.int32)
+    if a.dtype.kind not in "iu":
+        raise ValueError(f"{name} must hold integers, not {a.dtype}")
+    low, high = int(a.min()), int(a.max())
+    if low < 0 or high > 0x7FFFFFFF:
+        raise ValueError(f"{name} holds page {low if low < 0 else high}")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 class _Sequence:
     __slots__ = ("pages", "length")
 
@@ -63,10 +77,9 @@ class KVPagePool:
     # ---- device ---------------------------------------------------------------
     def copy_pages(self, src, dst, stream=None) -> None:
         """Page ``dst[i]`` becomes a copy of page ``src[i]`` in every cache.  A page
-        written twice, or both read and written, is a ``ValueError``.  (The
-        sequences' tables do not change.)"""
-        src = np.ascontiguousarray(src, dtype=np.int32)
-        dst = np.ascontiguousarray(dst, dtype=np.int32)
+        written twice, or both read and written, or a number that is no page of the
+        cache, is a ``ValueError``.  (The sequences' tables do not change.)"""
+        src, dst = _page_numbers("src", src), _page_numbers("dst", dst)
         if src.ndim != 1 or src.shape != dst.shape:
             raise ValueError("src and dst must be lists of one length")
         if src.size == 0:

@@ -134,6 +134,27 @@ def test_copy_pages(kw):
     assert _lib.last_error().startswith("copy_pages")
 
 
+@pytest.mark.parametrize("pages", [
+    np.array([2 ** 32 + 1, 2]), np.array([2 ** 31]), np.array([1.0, 2.0]), [1.5], [2 ** 40],
+    [2 ** 70], np.array([-2 ** 32]), [-1], [True], np.array([2 ** 63], dtype=np.uint64), ["1"]])
+def test_page_numbers_are_not_cast(pages):
+    from ie_tpq.kv_pages import KVPagePool
+
+    pool = KVPagePool.__new__(KVPagePool)     # its copy_pages refuses before it needs a cache
+    with pytest.raises(ValueError):
+        pool.copy_pages(pages, pages)
+
+
+def test_page_numbers_of_any_integer_type():
+    from ie_tpq.kv_pages import _page_numbers
+
+    for pages in ([3, 0, 2], (3, 0, 2), np.array([3, 0, 2], dtype=np.uint8),
+                  np.array([3, 9, 0, 9, 2], dtype=np.int64)[::2], np.array([3, 0, 2], dtype=">i4")):
+        got = _page_numbers("src", pages)
+        assert got.dtype == np.int32 and got.flags.c_contiguous and got.tolist() == [3, 0, 2]
+    assert _page_numbers("src", []).shape == (0,)
+
+
 def logprobs(**kw):
     a = dict(logits=4096, ld=100, dtype=_lib.IE_DT_F32, rows=2, vocab=100, tokens=4096, top=5,
              logprobs=4096, entropy=4096, top_logprobs=4096, top_tokens=4096, stream=None)
