@@ -34,14 +34,14 @@ class Continuation:
         return float(np.mean(self.logprobs)) if self.logprobs else 0.0
 
 
-def _sample(logits, temperature: float, generator):
+def _sample(model, logits, temperature: float, generator):
     """One token per row: the first maximum, or the exponential race over
-    softmax(logits / T)."""
+    softmax(logits / T).  Drawn tokens are rank 0's on every rank."""
     if temperature <= 0.0:
         return logits.argmax(dim=-1)
     probs = torch.softmax(logits / temperature, dim=-1)
     race = torch.empty_like(probs).exponential_(1.0, generator=generator).clamp_min(1e-10)
-    return (probs / race).argmax(dim=-1)
+    return model.of_rank0((probs / race).argmax(dim=-1))
 
 
 def best_of(model, prompt: list[int], n: int, max_new_tokens: int, *, block_size: int = 16,
@@ -74,7 +74,7 @@ def best_of(model, prompt: list[int], n: int, max_new_tokens: int, *, block_size
     out = [Continuation() for _ in range(n)]
     live = list(range(n))            # continuation of each row of the batch
     for step in range(max_new_tokens):
-        tokens = _sample(logits, temperature, gen)
+        tokens = _sample(model, logits, temperature, gen)
         scores = token_logprobs(logits, tokens, top=top)
         ids = tokens.tolist()
         lp, ent = scores.logprobs.tolist(), scores.entropy.tolist()

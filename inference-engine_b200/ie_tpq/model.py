@@ -393,8 +393,16 @@ class QuantizedTransformer:
         race = torch.empty_like(probs).exponential_(1.0).clamp_min(1e-10)
         sampled = (probs / race).argmax(dim=-1)
         chosen = torch.where(greedy, logits.argmax(dim=-1), sampled)
-        if self.world > 1 and not bool(greedy.all()):
-            mine = chosen.to(torch.float32) if self.shard.rank == 0 else torch.zeros_like(
-                chosen, dtype=torch.float32)
-            chosen = self.comm.all_reduce(mine).round().long()
+        if not bool(greedy.all()):
+            chosen = self.of_rank0(chosen)
         return chosen.tolist()
+
+    def of_rank0(self, chosen) -> "torch.Tensor":
+        """Rank 0's tokens on every rank (its own, and zeros from the others, summed)."""
+        import torch
+
+        if self.world == 1:
+            return chosen
+        mine = chosen.to(torch.float32) if self.shard.rank == 0 else torch.zeros_like(
+            chosen, dtype=torch.float32)
+        return self.comm.all_reduce(mine).round().long()

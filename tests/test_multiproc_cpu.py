@@ -114,3 +114,58 @@ def test_two_gloo_ranks_shard_and_reduce_in_rank_order():
             pass
     except mp.ProcessRaisedException as e:   # a rank's assertion, with its traceback
         pytest.fail(str(e))
+
+
+def _drawing_rank(rank: int, port: int, world: int) -> None:
+    import datetime
+    from types import SimpleNamespace
+
+    import torch
+    import torch.distributed as dist
+
+    from ie_tpq.best_of import _sample
+    from ie_tpq.model import QuantizedTransformer
+    from ie_tpq.sharding import Shard
+
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world,
+                            timeout=datetime.timedelta(seconds=60))
+    try:
+        def all_reduce(x):
+            dist.all_reduce(x)
+            return x
+
+        model = QuantizedTransformer.__new__(QuantizedTransformer)
+        model.shard, model.world = Shard(rank, world), world
+        model.comm = SimpleNamespace(all_reduce=all_reduce)
+        # ranks whose logits and draws are not the same
+        gen = torch.Generator().manual_seed(rank)
+        logits = torch.randn((6, 1000), generator=gen)
+        for temperature in (0.7, 2.0):
+            mine = _sample(model, logits, temperature, gen)
+            every = [torch.empty_like(mine) for _ in range(world)]
+            dist.all_gather(every, mine)
+            assert all(torch.equal(e, every[0]) for e in every)
+            if rank == 0:       # rank 0's own draw, not a mixture
+                again = torch.Generator().manual_seed(0)
+                torch.randn((6, 1000), generator=again)
+                if temperature == 0.7:
+                    one = QuantizedTransformer.__new__(QuantizedTransformer)
+                    one.world = 1
+                    assert torch.equal(mine, _sample(one, logits, temperature, again))
+        dist.barrier()
+    finally:
+        dist.destroy_process_group()
+
+
+def test_ranks_of_best_of_continue_with_rank_0s_draws():
+    import torch.multiprocessing as mp
+
+    ctx = mp.start_processes(_drawing_rank, args=(_free_port(), WORLD), nprocs=WORLD,
+                             join=False, start_method="spawn")
+    try:
+        while not ctx.join(timeout=120):
+            pass
+    except mp.ProcessRaisedException as e:
+        pytest.fail(str(e))
