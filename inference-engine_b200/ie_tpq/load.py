@@ -202,8 +202,30 @@ def read_config(directory) -> dict:
     return json.loads(path.read_text())
 
 
+def windows_from_hf(raw: dict) -> tuple[int, ...] | None:
+    """The attention window of each layer that a config.json declares, or None.
+
+    ``sliding_window`` counts where ``use_sliding_window`` does not switch it off (Llama
+    checkpoints have no windows, whatever the key says), in the layers that
+    ``layer_types`` names or, without it, from ``max_window_layers`` on (28 is the default
+    of the family that has ``use_sliding_window``; others have the window in every layer)."""
+    layers, size = raw["num_hidden_layers"], raw.get("sliding_window")
+    family = raw.get("model_type") or "".join(raw.get("architectures") or ())
+    if not size or not raw.get("use_sliding_window", not family.lower().startswith("llama")):
+        return None
+    types = raw.get("layer_types")
+    if types is None:
+        first = raw.get("max_window_layers", 28 if "use_sliding_window" in raw else 0)
+        types = ["full_attention" if i < first else "sliding_attention" for i in range(layers)]
+    if len(types) != layers or set(types) - {"full_attention", "sliding_attention"}:
+        raise ValueError(f"layer_types of {layers} layers: {types}")
+    windows = tuple(int(size) if t == "sliding_attention" else 0 for t in types)
+    return windows if any(windows) else None
+
+
 def config_from_hf(raw: dict):
-    """ie/load/huggingface.py:31-47 (rotary embedding halved, as HF stores it)."""
+    """ie/load/huggingface.py:31-47 (rotary embedding halved, as HF stores it), and the
+    layers' attention windows, which the reference does not read."""
     from .model import DecoderConfig
 
     heads = raw["num_attention_heads"]
@@ -214,7 +236,8 @@ def config_from_hf(raw: dict):
         num_heads=heads, num_kv_heads=raw.get("num_key_value_heads", heads),
         head_dim=raw.get("head_dim", hidden // heads), intermediate_size=raw["intermediate_size"],
         max_position=raw.get("max_position_embeddings", 4096), rope_base=float(rope),
-        norm_eps=float(raw.get("rms_norm_eps", 1e-6)), rope_halved=True)
+        norm_eps=float(raw.get("rms_norm_eps", 1e-6)), rope_halved=True,
+        windows=windows_from_hf(raw))
 
 
 def layer_names(index: int) -> dict[str, str]:
@@ -325,4 +348,4 @@ def load_quantized(directory, scheme: str = "int8", *, axis: int | None = 0, sha
 
 
 __all__ = ["SafetensorsFile", "ShardedCheckpoint", "open_checkpoint", "write_safetensors",
-           "read_config", "config_from_hf", "layer_names", "LoadReport", "load_quantized"]
+           "read_config", "config_from_hf", "windows_from_hf", "layer_names", "LoadReport", "load_quantized"]

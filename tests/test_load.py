@@ -164,3 +164,80 @@ def test_loaded_model_matches_the_oracle_and_the_in_memory_model(tmp_path, schem
     mem = QuantizedTransformer(src, scheme=scheme, dtype=torch.float32)
     prompts = [[1, 5, 9, 2], [7, 3]]
     assert greedy_generate(model, prompts, 6) == greedy_generate(mem, prompts, 6)
+
+
+FULL, SLIDING = "full_attention", "sliding_attention"
+
+
+@pytest.mark.parametrize("extra,windows", [
+    ({}, None),
+    # a window in every layer; switched off by null or by the flag
+    (dict(sliding_window=9), (9, 9, 9)),
+    (dict(sliding_window=None), None),
+    (dict(sliding_window=9, use_sliding_window=False), None),
+    (dict(sliding_window=9, use_sliding_window=False, layer_types=[FULL, SLIDING, FULL]), None),
+    # from a layer on
+    (dict(sliding_window=9, use_sliding_window=True, max_window_layers=1), (0, 9, 9)),
+    (dict(sliding_window=9, use_sliding_window=True, max_window_layers=0), (9, 9, 9)),
+    (dict(sliding_window=9, use_sliding_window=True, max_window_layers=3), None),
+    (dict(sliding_window=9, use_sliding_window=True), None),
+    # layer by layer
+    (dict(sliding_window=9, layer_types=[FULL, SLIDING, FULL]), (0, 9, 0)),
+    (dict(sliding_window=9, use_sliding_window=True, max_window_layers=0,
+          layer_types=[FULL, SLIDING, FULL]), (0, 9, 0)),
+    (dict(sliding_window=9, layer_types=[FULL, FULL, FULL]), None),
+    # an architecture without windows
+    (dict(sliding_window=9, model_type="llama"), None),
+])
+def test_hf_config_windows(extra, windows):
+    raw = {**HF_CONFIG, "architectures": ["SomeForCausalLM"], "num_hidden_layers": 3, **extra}
+    assert config_from_hf(raw).windows == windows
+    assert config_from_hf({**HF_CONFIG, "sliding_window": 9}).windows is None
+
+
+@pytest.mark.parametrize("types", [[SLIDING], [SLIDING, "chunked_attention", FULL]])
+def test_hf_config_windows_refuses_other_layers(types):
+    raw = {**HF_CONFIG, "architectures": ["SomeForCausalLM"], "num_hidden_layers": 3,
+           "sliding_window": 9, "layer_types": types}
+    with pytest.raises(ValueError):
+        config_from_hf(raw)
+
+
+@pytest.mark.gpu
+def test_a_loaded_model_keeps_its_windows(tmp_path, monkeypatch):
+    """The window of a checkpoint's config reaches the attention: the logits are those of
+    attention from its definition in f64, and not those without the window."""
+    import torch
+
+    import ie_tpq.model
+    from ie_tpq.decode import Layout
+    from ie_tpq.load import load_quantized
+    from tests.attention_oracle import attention
+
+    raw = {**HF_CONFIG, "architectures": ["SomeForCausalLM"], "sliding_window": 7}
+    synthetic_checkpoint(tmp_path, raw)
+    model, _ = load_quantized(tmp_path, "int8", dtype=torch.float32)
+    assert model.windows == (7, 7)
+    n = 40
+    layout = Layout([(5 * i) % 96 for i in range(n)], list(range(n)), list(range(n)), [n], [n],
+                    [[0, 1, 2]], True)
+
+    def logits():
+        k, v = model.allocate_caches(3, 16)
+        hidden = model.forward(layout, k, v, 16)
+        return model.logits_on_device(hidden, [1] * n).double()
+
+    got = logits()
+
+    def plain(q, k, v, tables, ctx, block, *, window, sinks, cu_seqlens_q, scale, **_):
+        out, _, _ = attention(q, k, v, tables, ctx.tolist(), block, window=window, sinks=sinks,
+                              query=cu_seqlens_q.diff().tolist(), scale=scale)
+        return torch.from_numpy(out).to(q)
+
+    monkeypatch.setattr(ie_tpq.model, "window_attention", plain)
+    # f32 throughout: two layers of sums of a few hundred products
+    torch.testing.assert_close(got, logits(), rtol=1e-4, atol=1e-5)
+    model.windows = (0, 0)
+    without = logits()
+    torch.testing.assert_close(got[:7], without[:7], rtol=1e-4, atol=1e-5)
+    assert (got[20:] - without[20:]).abs().max() > 1e-3
