@@ -231,7 +231,8 @@ class QuantizedTransformer:
         attn, mlp = self.attn[i], self.mlp[i]
         paged = plan.get("paged")     # this layer reads the cache with the own kernels
         if self.windows[i] and paged is None:
-            raise ValueError("layers with a window need the plan that forward() makes")
+            raise ValueError("layers with a window need a plan with context_lens and tables "
+                             "(and cu_q for several queries a sequence)")
         own = paged is not None and (self.windows[i] > 0 or paged["prefix"] is not None)
         # A prefill of fresh prompts attends over its own k and v (not the
         # cache) and needs them as tensors; every other step reads the cache.
@@ -287,11 +288,27 @@ class QuantizedTransformer:
     def run(self, tokens, positions, block_tables, plan, layout, k_caches, v_caches,
             block_size: int):
         """ie/model/torch_transformer.py:92-98."""
+        if plan.get("paged") is None and any(self.windows):
+            plan = {**plan, "paged": self._paged_plan(plan, block_tables, layout)}
         x = self.embedding.index_select(0, tokens)
         for i in range(len(self.attn)):
             x = self._layer(i, x, positions, block_tables, plan, layout, k_caches[i],
                             v_caches[i], block_size)
         return rms_norm(x, self.final_norm, self.config.norm_eps)
+
+    def _paged_plan(self, plan, block_tables, layout):
+        """What ``window_attention`` takes, from a plan that ``forward`` did not make (a
+        captured decode step's): its lengths and tables on the device.  None where the
+        plan has none."""
+        torch = require_cuda()
+        lens, tables, cu_q = (plan.get(name) for name in ("context_lens", "tables32", "cu_q"))
+        if tables is None:
+            tables = block_tables
+        if lens is None or tables is None or (layout.max_query_len > 1 and cu_q is None):
+            return None
+        return {"prefix": None, "tables": tables.to(torch.int32),
+                "context_lens": lens.to(torch.int32),
+                "cu_q": cu_q.to(torch.int32) if layout.max_query_len > 1 else None}
 
     def forward(self, layout, k_caches, v_caches, block_size: int):
         """ie/model/torch_transformer.py:100-122."""

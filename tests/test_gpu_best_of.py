@@ -166,3 +166,49 @@ def test_refusals():
         windowed.run(torch.zeros(1, dtype=torch.long, device="cuda"),
                      torch.zeros(1, dtype=torch.long, device="cuda"), None, {"flash": False},
                      None, k, v, 16)
+
+
+@pytest.mark.parametrize("windows", [(6, 5), (0, 7)])
+def test_a_windowed_model_runs_a_captured_decode_step(windows):
+    """``run`` with a plan of device tensors that a caller made, captured in a graph:
+    the steps of ``forward``, whole and windowed layers alike."""
+    model = QuantizedTransformer(source(windows, 2), scheme="int8", dtype=torch.float16)
+    block, n = 256, len(PROMPT)
+    long = dict(device="cuda", dtype=torch.long)
+    i32 = dict(device="cuda", dtype=torch.int32)
+
+    def prefilled():
+        k, v = model.allocate_caches(2, block)
+        layout = Layout(PROMPT + PROMPT, list(range(n)) * 2,
+                        [*range(n), *range(block, block + n)], [n, n], [n, n], [[0], [1]], True)
+        model.forward(layout, k, v, block)
+        return k, v
+
+    def layout_at(p):
+        return Layout([1, 2], [p, p], [p, block + p], [p + 1, p + 1], [1, 1], [[0], [1]], False)
+
+    k, v = prefilled()
+    want = [model.forward(layout_at(p), k, v, block).clone() for p in range(n, n + 4)]
+    k, v = prefilled()
+    tokens, positions = torch.tensor([1, 2], **long), torch.tensor([n, n], **long)
+    slots, lens = torch.tensor([n, block + n], **long), torch.tensor([n + 1, n + 1], **i32)
+    tables = torch.tensor([[0], [1]], **long)
+    plan = {"flash": True, "scale": 64 ** -0.5, "slots": slots, "context_lens": lens, "cu_q": None,
+            "cu_k": None, "paged_tables": None, "tables32": tables.to(torch.int32)}
+    step = lambda: model.run(tokens, positions, tables, plan, layout_at(n), k, v, block)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        graph.replay()
+        torch.testing.assert_close(out, want[i], rtol=2e-2, atol=2e-2)
+        for t in (positions, slots, lens):
+            t += 1
+    with pytest.raises(ValueError):
+        model.run(tokens, positions, tables, {**plan, "context_lens": None}, layout_at(n), k, v,
+                  block)
