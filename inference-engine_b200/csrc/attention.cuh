@@ -24,6 +24,13 @@ struct FastDiv {
   }
 };
 
+// The tensor-core kernels take a row's weights relative to 2^(its maximum - kBelow): an f16
+// weight keeps its 11 bits down to 2^-14, so 7 more binades of a long flat tail are
+// rounded like the rest (the raised-late maximum adds 2^8: 2^15 at most, below 65504).
+// bf16 has the exponents of f32.
+template <typename T> constexpr float kBelow = 0.0f;
+template <> constexpr float kBelow<__half> = 7.0f;
+
 struct Params {
   const void* q;
   const void* k;

@@ -226,7 +226,7 @@ attention_decode_kernel(const Params p, const int per) {
     for (int h = 0; h < 2; ++h) {
       mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 2)) * p.scale2;
+      mx[h] = fmaf(fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 2)), p.scale2, -kBelow<T>);
     }
     if (__any_sync(~0u, mx[0] > m[0] + kLazy || mx[1] > m[1] + kLazy)) {
 #pragma unroll

@@ -1053,7 +1053,8 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
         for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(raw[i]);
 #pragma unroll
         for (int i = 4; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(raw[i]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+        const float top =
+            fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), scale2, -kBelow<T>);
         if (__any_sync(~0u, top > m + kLazy)) {
           const float mn = fmaxf(m, top);
           const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);

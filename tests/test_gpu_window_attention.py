@@ -202,6 +202,31 @@ def test_large_scores(dtype):
     check(b)
 
 
+@pytest.mark.parametrize("dtype,hd", [(F16, 64), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("query", [None, [3]])
+def test_a_long_flat_tail(dtype, hd, query):
+    """A key of weight 1 before some 65000 of 2.48 * 2^-24, 1 % of the sum: an f16 weight
+    that small is off by a fifth (two bounds of the sum), unless it is taken relative to a
+    smaller maximum.  The lengths given make the rows one part; of one query's eight warps
+    each has its large key and its tail.  (With more keys the f32 sums' own roundings, of a
+    sixteen keys' 2^-19 beside 1, come near the bound.)"""
+    context, peaks = (520000, torch.arange(0, 128, 16)) if query is None else (70000, [0])
+    b = Batch([context], 2, 1, hd, dtype, 256, query=query, seed=18, spare=0)
+    b.q.zero_()
+    b.q[:, :, 0] = hd ** 0.5                    # a score is the key's first element
+    first = int(b.tables[0, 0]) * 256
+    b.k.zero_()
+    b.k[:, :, 0] = -15.7266
+    b.v = (b.v.nan_to_num(0.0).float() * 0.1 + 1).to(dtype)
+    for at in peaks:
+        b.k[first + int(at)] = 0.0
+        b.v[first + int(at)] = -1.0
+    got = window_attention(b.q, b.k, b.v, b.tables, b.ctx, 256, cu_seqlens_q=b.cu,
+                           max_query_len=3, max_context_len=64)
+    want, weight, largest = b.oracle()
+    assert_close(got, want, weight, largest, hd)
+
+
 def test_strides():
     """q as a slice of the fused projection, caches as halves of one tensor, a table
     that is a slice, and an output with wider rows."""
