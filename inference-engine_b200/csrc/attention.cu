@@ -263,13 +263,13 @@ Plan make_plan(const ie_attention_args& a) {
   return plan;
 }
 
-// The workspace: the parts' sums in f32, then their (m, l) pairs, which start on an
-// 8-byte boundary whatever the head size.
+// The workspace: the parts' sums in f32 from the first 32-byte boundary on (the tiles
+// store that many), then their (m, l) pairs, 8-byte aligned whatever the head size.
 size_t part_sums(const ie_attention_args& a, int slots) {
   return ((size_t)a.tokens * a.heads * slots * a.head_dim + 1) / 2 * 2;
 }
 size_t part_bytes(const ie_attention_args& a, int slots) {
-  return part_sums(a, slots) * 4 + (size_t)a.tokens * a.heads * slots * 8;
+  return slots ? 16 + part_sums(a, slots) * 4 + (size_t)a.tokens * a.heads * slots * 8 : 0;
 }
 
 int run(const ie_attention_args& a, void* workspace, size_t workspace_bytes, const char* who,
@@ -282,7 +282,7 @@ int run(const ie_attention_args& a, void* workspace, size_t workspace_bytes, con
   Params p = base_params(a);
   p.prefix = (int)std::min<int64_t>(a.prefix_len, 0x7FFFFFFF);
   p.slots = plan.slots;
-  p.part_o = static_cast<float*>(workspace);
+  p.part_o = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 31) / 32 * 32);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + part_sums(a, plan.slots));
   if (plan.simt) {
     p.parts = plan.simt_parts;

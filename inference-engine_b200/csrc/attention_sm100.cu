@@ -94,7 +94,6 @@ struct TileParams {
   int per_tile;      // tokens of a row tile: 128 / group
   int row_tiles;     // work tiles (two row tiles, one when twin) of a segment in the grid
   bool wide_out;     // out rows are 32-byte aligned
-  bool wide_part;    // part_o is (a workspace is 16-byte aligned, no more)
   int segs;          // sequences (prefill) or 1 (prefix)
   int parts;         // key parts of a work tile
 };
@@ -1133,7 +1132,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
         }
         if (live && p.slots) {
 #pragma unroll
-          for (int i = 0; i < 64; i += 8) store32(p.part_o + at * HD + h + i, o + i, a.wide_part);
+          for (int i = 0; i < 64; i += 8) store32(p.part_o + at * HD + h + i, o + i, true);
         } else if (live) {
 #pragma unroll
           for (int i = 0; i < 64; i += 16) {
@@ -1344,7 +1343,6 @@ int launch_tiles(const Params& p, int dtype, bool prefix, bool twin, int row_til
   a.segs = prefix ? 1 : p.seqs;
   a.parts = parts;
   a.wide_out = (reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_token * 2) % 32 == 0;
-  a.wide_part = reinterpret_cast<uintptr_t>(p.part_o) % 32 == 0;
   return dtype == IE_DT_BF16 ? launch<__nv_bfloat16>(a, dtype, s) : launch<__half>(a, dtype, s);
 }
 

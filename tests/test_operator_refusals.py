@@ -97,7 +97,7 @@ def test_odd_head_sizes_leave_room_for_aligned_pairs(head_dim):
              q_head_stride=head_dim, out_token_stride=head_dim, slot_stride=head_dim,
              head_stride=head_dim, dtype=_lib.IE_DT_F32, table_width=12, table_stride=12)
     need = _lib.lib().ie_attention_workspace_size(ctypes.byref(a))     # three parts
-    assert need == (3 * head_dim + 1) * 4 + 3 * 8
+    assert need == 16 + (3 * head_dim + 1) * 4 + 3 * 8
 
 
 def test_nothing_to_do_is_not_an_error():
