@@ -121,28 +121,23 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// What the roles tell one another: that one has given up, and (a count that moves) that
-// rows are being computed again, for which the others wait as long as it takes.
+// What the roles tell one another: that one has given up, and when (clock64) rows were
+// last being computed again, for which the others wait as long as it takes.
 struct Signals {
-  int quit, beat;
+  long long beat;
+  int quit;
 };
 // False once the limit has passed without a beat or another role has given up.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile Signals* x) {
   if (mbar_try(bar, parity)) return true;
-  long long t0 = clock64();
-  int beat = x->beat;
+  const long long t0 = clock64();
   while (true) {
     if (mbar_try(bar, parity)) return true;
     if (x->quit) return false;
-    if (clock64() - t0 > kWaitCycles) {
-      const int now = x->beat;
-      if (now == beat) {
-        atomicOr(&g_attention_status, 1u);
-        x->quit = 1;
-        return false;
-      }
-      beat = now;
-      t0 = clock64();
+    if (clock64() - t0 > kWaitCycles && clock64() - x->beat > kWaitCycles) {
+      atomicOr(&g_attention_status, 1u);
+      x->quit = 1;
+      return false;
     }
   }
 }
@@ -478,7 +473,7 @@ __device__ __forceinline__ bool keys_of_row(const TileParams& a, const Work& w, 
     const int v0 = j * kTile;
     if (unseen && see.tile(a.p, v0)) continue;
     for (int i = 0; i < kTile && v0 + i < w.n; i += 32) {
-      if (lane == 0) atomicAdd(&c->signals.beat, 1);
+      if (lane == 0) *static_cast<volatile long long*>(&c->signals.beat) = clock64();
       const int v = v0 + i + lane;
       if (f(v, see.one(a.p, v))) return true;
     }
@@ -571,6 +566,35 @@ __device__ __noinline__ void row_again(const TileParams& a, const Work& w, Contr
     for (int e = 0; e < HD / 32; ++e) over = over && o[e] != o[e];
     return __all_sync(~0u, over) != 0;
   });
+}
+
+// Warp-wide: those of the lanes' rows that `again` names are computed again where they are
+// spoilt, and written over their first result.
+template <typename T, int HD>
+__device__ __noinline__ void mend_rows(const TileParams& a, const Work& w, Control* c,
+                                       uint32_t again, int t, int head, int pos, int stream,
+                                       int slot, float m, float l) {
+  const Params& p = a.p;
+  const int lane = threadIdx.x & 31;
+  __syncwarp();       // the rows' own stores come before what other lanes write
+  while (again) {
+    const int src = __ffs(again) - 1;
+    again &= again - 1;
+    const int tt = __shfl_sync(~0u, t, src), hh = __shfl_sync(~0u, head, src);
+    const int pp = __shfl_sync(~0u, pos, src);
+    const float mm = __shfl_sync(~0u, m, src), ll = __shfl_sync(~0u, l, src);
+    if (!spoilt<T, HD>(a, w, c, pp, stream)) continue;     // what it sees is not finite
+    float o[HD / 32];
+    row_again<T, HD>(a, w, c, tt, hh, pp, stream, mm, o);
+    const int64_t at = ((int64_t)tt * p.heads + hh) * p.slots + slot;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) {
+      if (p.slots) p.part_o[at * HD + lane + 32 * e] = o[e];
+      else
+        static_cast<T*>(p.out)[(int64_t)tt * p.out_token + (int64_t)hh * HD + lane + 32 * e] =
+            from_f32<T>(o[e] / ll);
+    }
+  }
 }
 
 // 32 bytes of a thread's own row: a whole sector a store where the row allows it
@@ -989,7 +1013,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c,
 template <typename T, int HD>
 __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int s) {
   const Params& p = a.p;
-  const int r = threadIdx.x & (kTile - 1), lane = threadIdx.x & 31;
+  const int r = threadIdx.x & (kTile - 1);
   const uint32_t lanes = (uint32_t)(r & ~31) << 16;       // this warp's TMEM lanes
   const uint32_t ts = tmem + lanes + s * kTile, to = tmem + lanes + 2 * kTile + s * HD;
   const float scale2 = p.scale2;
@@ -1148,26 +1172,8 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
       if (live && p.slots) p.part_ml[at] = make_float2(m, l);
 
       // a sum that is not finite is the row's own: only keys that it sees enter it
-      uint32_t again = __ballot_sync(~0u, live && l - l == 0.0f && !(check == 0.0f));
-      if (again) __syncwarp();       // the rows' own stores come before what other lanes write
-      while (again) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        const int tt = __shfl_sync(~0u, t, src), hh = __shfl_sync(~0u, head, src);
-        const int pp = __shfl_sync(~0u, pos, src);
-        const float mm = __shfl_sync(~0u, m, src), ll = __shfl_sync(~0u, l, src);
-        if (!spoilt<T, HD>(a, w, c, pp, s)) continue;     // what it sees is not finite
-        float o[HD / 32];
-        row_again<T, HD>(a, w, c, tt, hh, pp, s, mm, o);
-        const int64_t at2 = ((int64_t)tt * p.heads + hh) * p.slots + slot;
-#pragma unroll
-        for (int e = 0; e < HD / 32; ++e) {
-          if (p.slots) p.part_o[at2 * HD + lane + 32 * e] = o[e];
-          else
-            static_cast<T*>(p.out)[(int64_t)tt * p.out_token + (int64_t)hh * HD + lane + 32 * e] =
-                from_f32<T>(o[e] / ll);
-        }
-      }
+      const uint32_t again = __ballot_sync(~0u, live && l - l == 0.0f && !(check == 0.0f));
+      if (again) mend_rows<T, HD>(a, w, c, again, t, head, pos, s, slot, m, l);
     }
   }
 }
@@ -1197,7 +1203,8 @@ attention_tile_kernel(const __grid_constant__ TileParams a, const __grid_constan
     mbar_init(smem_u32(&c->q_free), 1);
     mbar_init(smem_u32(&c->next_full), 1);
     mbar_init(smem_u32(&c->next_empty), W::kReaders);
-    c->signals = Signals{0, 0};
+    c->signals.beat = 0;
+    c->signals.quit = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == W::kIssue) {
