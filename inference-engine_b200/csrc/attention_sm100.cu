@@ -378,8 +378,7 @@ __device__ __forceinline__ void ask_next(Control* c, uint32_t n) {
 // its virtual keys.  Every role derives it alike.
 struct Work {
   int seg, kvh, part, first;
-  int tok0, ctx, ntok;                 // of the segment: first token, context, tokens
-  int begin, end;                      // its sequence's own tokens (see `segment`)
+  int tok0, ntok, pos0;                // of the segment: first token, tokens, first position
   int lo, ns, n;                       // virtual keys: ns sinks, then from lo
   int j0, j1;
 };
@@ -402,19 +401,15 @@ __device__ __forceinline__ bool segment(const TileParams& a, int item, Work& w, 
   w.part = item % a.parts;
   tile = a.row_tiles - 1 - item / a.parts;      // the longest contexts first
   if (a.mode == kPrefix) {
-    w.tok0 = w.begin = 0;
-    w.ntok = w.end = p.tokens;
-    w.ctx = 0;
+    w.tok0 = w.pos0 = 0;
+    w.ntok = p.tokens;
   } else {
-    w.begin = p.cu_q ? __ldg(p.cu_q + w.seg) : w.seg;
-    w.end = p.cu_q ? __ldg(p.cu_q + w.seg + 1) : w.seg + 1;
-    // the first and the last segment take in the tokens that are no sequence's, whose rows
-    // see nothing and are zeros
-    w.tok0 = w.seg == 0 ? 0 : w.begin;
-    w.ntok = (w.seg == a.segs - 1 ? p.tokens : min(w.end, p.tokens)) - w.tok0;
-    // a table of lengths that does not begin in [0, tokens] reads and writes nothing
-    if (w.begin < 0 || w.begin > p.tokens) w.ntok = 0;
-    w.ctx = context_of(p, w.seg);
+    w.tok0 = p.cu_q ? __ldg(p.cu_q + w.seg) : w.seg;
+    w.ntok = p.cu_q ? __ldg(p.cu_q + w.seg + 1) - w.tok0 : 1;
+    w.pos0 = context_of(p, w.seg) - w.ntok;
+    // a table of lengths that does not describe [0, tokens) reads and writes nothing
+    if (w.tok0 < 0 || w.tok0 > p.tokens) w.ntok = 0;
+    w.ntok = min(w.ntok, p.tokens - w.tok0);
   }
   return w.ntok > tile * tokens_of_work(a);
 }
@@ -425,11 +420,8 @@ __device__ __forceinline__ void locate(const TileParams& a, Work& w, int tile) {
     w.lo = w.ns = 0;
     w.n = p.key_end;
   } else {
-    // the sequence's tokens among the tile's
-    const int t0 = max(w.tok0 + w.first, w.begin);
-    const int t1 = min(w.tok0 + min(w.first + tokens_of_work(a), w.ntok), w.end) - 1;
-    const int first = max(w.ctx - (w.end - t0), 0);
-    const int last = t0 > t1 ? -1 : w.ctx - (w.end - t1);
+    const int first = max(w.pos0 + w.first, 0);
+    const int last = w.pos0 + min(w.first + tokens_of_work(a), w.ntok) - 1;
     w.lo = p.key_start;
     if (p.window > 0) w.lo = max(w.lo, first - p.window + 1);
     w.ns = p.key_start == 0 ? min(p.sinks, w.lo) : 0;
@@ -443,6 +435,35 @@ __device__ __forceinline__ void locate(const TileParams& a, Work& w, int tile) {
   const int tiles = (w.n + kTile - 1) / kTile;
   w.j0 = (int)((int64_t)tiles * w.part / a.parts);
   w.j1 = (int)((int64_t)tiles * (w.part + 1) / a.parts);
+}
+
+// Rows of tokens that are no sequence's: those in front of the first sequence and behind
+// the last.  The softmax warps of that sequence's items write them, the chunks of tokens
+// spread over its items; whether the item has work of its own does not matter.
+template <typename T, int HD>
+__device__ __noinline__ void rows_of_no_sequence(const TileParams& a, const Work& w, int tile,
+                                                 int s) {
+  const Params& p = a.p;
+  if (!p.cu_q || (!a.twin && s > 0)) return;
+  const int step = tokens_of_work(a);
+  for (int side = 0; side < 2; ++side) {
+    if (w.seg != (side ? a.segs - 1 : 0)) continue;
+    const int at = min(max(__ldg(p.cu_q + (side ? a.segs : 0)), 0), p.tokens);
+    const int lo = side ? at : 0, hi = side ? p.tokens : at;
+    for (int64_t c = lo + (int64_t)tile * step; c < hi; c += (int64_t)a.row_tiles * step)
+      for (int r = threadIdx.x & (kTile - 1); r < min(step, hi - (int)c) * p.group; r += kTile) {
+        const int tok = p.group_div.div(r);
+        const int t = (int)c + tok, head = w.kvh * p.group + r - tok * p.group;
+        if (p.slots) {
+          const int slot = p.slot0 + w.part * (a.twin ? 2 : 1) + (a.twin ? s : 0);
+          p.part_ml[((int64_t)t * p.heads + head) * p.slots + slot] = make_float2(-INFINITY, 0.0f);
+        } else {
+          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_token +
+                                                (int64_t)head * HD);
+          for (int i = 0; i < HD / 8; ++i) out[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+  }
 }
 
 // ---- rows that a value behind their mask has spoilt (see the top) ------------------------
@@ -1025,7 +1046,11 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
   for (Items it(blockIdx.x); it.item >= 0; it.next(c)) {
     Work w;
     int tile;
-    if (!segment(a, it.item, w, tile)) continue;
+    const bool work = segment(a, it.item, w, tile);
+    if (a.mode == kPrefill && ((w.seg == 0 && w.tok0 > 0) ||
+                               (w.seg == a.segs - 1 && w.tok0 + w.ntok < p.tokens)))
+      rows_of_no_sequence<T, HD>(a, w, tile, s);
+    if (!work) continue;
     for (; tile * tokens_of_work(a) < w.ntok; tile += a.row_tiles) {
       locate(a, w, tile);
       const uint32_t tile0 = tiles;
@@ -1037,9 +1062,7 @@ __device__ void softmax_role(const TileParams& a, Control* c, uint32_t tmem, int
       const int head = w.kvh * p.group + row_head;
       int pos = -1;
       if (live) pos = a.mode == kPrefix ? position_of(p, sequence_of(p, t), t)
-                                        : t >= w.begin && t < w.end
-                                              ? max(w.ctx - (w.end - t), -1)
-                                              : -1;
+                                        : max(w.pos0 + tok, -1);
       const Seen seen(p, w, pos);
       const int vmax = seen.vmax, vmin = seen.vmin;
 
