@@ -255,7 +255,7 @@ struct Row {
 // reads the row twice: for the maximum, then for weights 2^((x - m) log2 e).  m itself is
 // not finite where the row has +inf or nothing above -inf, and the sums are then NaN.
 template <typename T, int kThreads>
-__device__ __noinline__ Sums far_sums(const Row<T, kThreads>& row, float* shared) {
+__device__ Sums far_sums(const Row<T, kThreads>& row, float* shared) {
   constexpr int kPer = Vec<T>::kPer, kWarps = kThreads / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float m = -INFINITY;
