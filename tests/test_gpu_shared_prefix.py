@@ -173,3 +173,18 @@ def test_refusals():
     with pytest.raises(ValueError):
         shared_prefix_attention(b.q[:1], *args[1:], 32, 16)
     assert np.isfinite(b.q.float().cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("block", [1, 5, 20, 48, 256])
+@pytest.mark.parametrize("heads,kv,hd,dtype", [(16, 8, 128, BF16), (8, 4, 64, F16)])
+@pytest.mark.parametrize("query", [None, [3, 1, 40, 0, 17]])
+def test_pages_of_any_size(block, heads, kv, hd, dtype, query):
+    """A prefix long enough for the row tiles, in pages that are gathered or taken in boxes."""
+    if query is None:
+        b = Batch([1301 + 3 * i for i in range(40)], heads, kv, hd, dtype, block, prefix=1300,
+                  seed=block)
+        b.context[1], b.ctx[1] = 700, 700
+    else:
+        b = Batch([1300 + n for n in (9, 1, 40, 0, 90)], heads, kv, hd, dtype, block, query=query,
+                  prefix=1300, seed=block)
+    assert torch.equal(check(b), check(b))

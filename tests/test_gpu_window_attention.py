@@ -468,3 +468,55 @@ def test_odd_head_sizes_split_into_parts(hd, dtype):
         assert _lib.lib().ie_attention_workspace_size(ctypes.byref(c_args(b, out))) > 0
         check(b)
         check(b, window=150, sinks=3)
+
+
+def workspace(b, **kw):
+    return _lib.lib().ie_attention_workspace_size(ctypes.byref(c_args(b, torch.empty_like(b.q),
+                                                                      **kw)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("context,heads,kv,hd", [
+    ([20001], 4, 1, 128), ([20000, 0], 2, 2, 64), ([9973, 20003], 3, 1, 128),
+    ([30000, 5], 20, 1, 64)])
+def test_decode_rows_in_parts_and_their_join(dtype, context, heads, kv, hd):
+    """Rows long enough to go through the workspace, beside short and empty ones."""
+    b = Batch(context, heads, kv, hd, dtype, 16, seed=hd)
+    assert workspace(b) > 0 and workspace(b, window=15000, sinks=4) > 0
+    check(b)
+    check(b, window=15000, sinks=4)
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("seqs", [38, 56, 74])
+def test_decode_of_a_batch_that_a_window_makes_even(dtype, hd, seqs):
+    """297 to 592 rows of one part: CTAs of two warps."""
+    b = Batch([64 + 5 * i for i in range(seqs)], 16, 8, hd, dtype, 16, seed=seqs)
+    b.context[3] = 0
+    b.ctx[3] = 0
+    assert workspace(b, window=48, sinks=2) == 0
+    check(b, window=48, sinks=2)
+    check(b, window=17)
+
+
+@pytest.mark.parametrize("seqs,kv", [(1, 4), (2, 8), (3, 8), (5, 8), (9, 8), (20, 8), (40, 8)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_in_clusters_of_every_size(seqs, kv, hd):
+    check(Batch([1500 - 3 * i for i in range(seqs)], kv, kv, hd, BF16, 16, seed=seqs))
+
+
+@pytest.mark.parametrize("heads,kv", [(130, 1), (260, 2)])
+@pytest.mark.parametrize("query", [None, [9, 3]])
+def test_more_than_128_query_heads_a_kv_head(heads, kv, query):
+    b = Batch([200, 77], heads, kv, 64, BF16, 16, query=query, seed=heads)
+    check(b)
+    check(b, window=60, sinks=3)
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("block", [1, 3, 5, 20, 24, 40, 96])
+def test_pages_of_any_size_under_row_tiles(dtype, hd, block):
+    """Pages that no TMA box fits are gathered; others take boxes of 8, 16 or 32 rows."""
+    b = Batch([100, 1000, 300], 4, 2, hd, dtype, block, query=[100, 3, 260], seed=block)
+    check(b)
+    check(b, window=90, sinks=4)
