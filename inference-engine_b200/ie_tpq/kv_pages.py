@@ -30,6 +30,8 @@ def _page_numbers(name: str, pages) -> np.ndarray:
     """A list or array of page numbers as int32; what int32 cannot hold as it is (floats,
     numbers beyond its range) is refused, not cast."""
     a = np.asarray(pages)
+    if a.dtype == np.int32:          # the library checks the range
+        return np.ascontiguousarray(a)
     if a.size == 0:
         return np.zeros(a.shape, dtype=np.int32)
     if a.dtype.kind not in "iu":
