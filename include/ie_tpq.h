@@ -264,13 +264,15 @@ int ie_rope_kv(const void* qkv, int64_t ld_qkv, int32_t dtype, int64_t tokens, i
  * (window == 0 or j > p - window or j < sinks).
  * ie_shared_prefix_attention: j <= p, where the keys below prefix_len are the
  * same for every sequence and are looked up in the FIRST row of block_tables;
- * they are read once for the whole batch (a short prefix once a sequence, from L2).
+ * they are read once for the whole batch (a short prefix once a sequence, from L2, and
+ * so is any prefix by the CUDA cores, see below).
  *
  * Both: a query that sees nothing (an empty context, or a token in front of
  * cu_seqlens_q[0] or from cu_seqlens_q[seqs] on, which is no sequence's) gets zeros.  A key whose
  * table entry names no page of the cache (-1, as a page given back reads) is not
  * seen; K and V rows that are not seen may hold anything, NaN included.
- * Softmax, sums and the join of parts are f32.  f32 rows, head sizes other than
+ * Softmax, sums and the join of parts are f32; 16-bit types round a softmax weight once
+ * before it meets V.  `out` must not overlap the inputs.  f32 rows, head sizes other than
  * 64 and 128 and rows that are not 16-byte aligned run on the CUDA cores. */
 #define IE_ATTENTION_MAX_HEAD_DIM 256
 typedef struct ie_attention_args {

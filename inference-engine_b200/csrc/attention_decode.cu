@@ -17,12 +17,17 @@
 // path, the eight warps of an SM (two CTAs of four, one of eight where there are no
 // more CTAs than SMs, or four of two) keep 128 KB of loads in flight, and pages of
 // any size cost one table lookup per key.  64 sequences, heads 32/8 x 128, window
-// 4096 take 151 us, 6.6 TB/s; one sequence, window 1024, 6.6 us.
+// 4096 take 153 us in a graph, 6.5 TB/s; one sequence, window 1024, 7.1 us.
 //
 // The maximum is raised only when a score passes it by more than 2^8: the sums
 // stay far inside f32 and the outputs are rescaled a few times a row instead of
 // every step.  Weights are rounded to the element type for the product with
-// V, the rounding that the tensor cores' operands impose; their sum is not.
+// V, the rounding that the tensor cores' operands impose; their sum is not.  A second
+// product with what the rounding left would take the error of the output from that of two
+// roundings to one (bf16: 2.3e-3 and 1.7e-3 of its norm); it cost 3 % at 64 sequences,
+// window 4096 (151 and 156 us), 7 % at 64 of up to 4096 (105 and 113) and 11 % at 8 of up
+// to 8192 (37 and 42), and is not made.  An f16 weight keeps its bits down to 2^-21 of the
+// row's largest (kBelow).
 //
 // A few parts of a row form a thread-block cluster and are joined through
 // distributed shared memory: one launch, no workspace.  A short prefix that the

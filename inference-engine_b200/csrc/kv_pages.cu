@@ -5,7 +5,7 @@
 // 2 * pages * page bytes at the copy bandwidth.  A CTA moves 16 KB of one page of one
 // cache (256 threads x four 16-byte vectors, all loaded before the first store);
 // eight are resident on an SM, 128 KB of loads in flight.  220 pages of 32 KB in 64
-// caches take 138 us, 6.7 TB/s; CTAs that stay and stride over the units took 160, as
+// caches take 140 us, 6.6 TB/s; CTAs that stay and stride over the units took 160, as
 // each waits for its own stores before it loads again.
 //
 // The page numbers and the cache addresses travel as kernel parameters (up to

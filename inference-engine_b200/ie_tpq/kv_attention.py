@@ -144,8 +144,9 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, pre
                             stream=None):
     """Causal attention of sequences that begin with the same ``prefix_len`` tokens:
     the prefix is read through the first row of ``block_tables``, once for the
-    whole batch (a short prefix of few sequences: by each, from L2), and the keys from ``prefix_len`` on through each
-    sequence's own row.  A sequence shorter than the prefix sees its part of
+    whole batch (a short prefix of few sequences, and any prefix in f32 or with other head
+    sizes than 64 and 128: by each, from L2), and the keys from ``prefix_len`` on through
+    each sequence's own row.  A sequence shorter than the prefix sees its part of
     it.  The other arguments are those of ``window_attention``."""
     return _attend("ie_shared_prefix_attention", q, k_cache, v_cache, block_tables, context_lens,
                    block_size, 0, 0, prefix_len, cu_seqlens_q, max_query_len, max_context_len,
