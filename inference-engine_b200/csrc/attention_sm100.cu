@@ -48,9 +48,9 @@
 // keys that the row met but does not see; where it finds such a value, it computes the
 // row's output again over the keys that the row sees.
 //
-// Every wait has a limit, counted from the last sign that rows are being computed again
-// (which takes time in proportion to their contexts); a wait that runs out sets an error
-// bit (ie_kernel_status) and all roles leave.
+// Every wait has a limit, counted from the last sign that a long item's key tiles go on or
+// rows are being computed again (both take time in proportion to their contexts); a wait
+// that runs out sets an error bit (ie_kernel_status) and all roles leave.
 #include <cuda.h>
 
 #include <mutex>
@@ -69,6 +69,7 @@ constexpr float kLazy = 8.0f;
 // 2 x 8192 tokens, window 2048); larger ones than 32 only add masked keys to the window.
 constexpr int kMaxBox = 32;
 constexpr long long kWaitCycles = 4000000000ll;   // ~2 s
+constexpr int kBeatTiles = 4096;   // key tiles between two signs of a long item, some 10 ms
 constexpr int kInvalidRing = 8;
 
 __device__ uint32_t g_attention_status = 0;
@@ -122,8 +123,9 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// What the roles tell one another: that one has given up, and when (clock64) rows were
-// last being computed again, for which the others wait as long as it takes.
+// What the roles tell one another: that one has given up, and when (clock64) key tiles of a
+// long item were last issued or rows being computed again, for which the others wait
+// as long as it takes.
 struct Signals {
   long long beat;
   int quit;
@@ -145,6 +147,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // The same for a whole warp: all lanes get one answer.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile Signals* x) {
   return __all_sync(~0u, mbar_wait(bar, parity, x));
+}
+__device__ __forceinline__ void beat(Signals& x) {
+  *static_cast<volatile long long*>(&x.beat) = clock64();
 }
 // True in one lane of a converged warp.  The instructions of the asynchronous units take
 // their operands from uniform registers: a whole warp runs the code around them
@@ -495,7 +500,7 @@ __device__ __forceinline__ bool keys_of_row(const TileParams& a, const Work& w, 
     const int v0 = j * kTile;
     if (unseen && see.tile(a.p, v0)) continue;
     for (int i = 0; i < kTile && v0 + i < w.n; i += 32) {
-      if (lane == 0) *static_cast<volatile long long*>(&c->signals.beat) = clock64();
+      if (lane == 0) beat(c->signals);
       const int v = v0 + i + lane;
       if (f(v, see.one(a.p, v))) return true;
     }
@@ -983,6 +988,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c,
         Cursor v[2];        // V tile of each stream's last scores
         for (int i = 0; i < nt + 2; ++i) {
           const int s = i & 1;
+          if (i % kBeatTiles == kBeatTiles - 1 && leader) beat(c->signals);
           if (i >= 2) {       // the product of step i - 2, the same stream
             const Cursor x = s ? v[1] : v[0];
             if (!full(x) || !product(s, x, i < 4)) return;
@@ -1005,6 +1011,7 @@ __device__ void issue_role(const TileParams& a, uint8_t* base, Control* c,
         const int streams = row_tiles_of(a, w);
         Cursor v;           // V tile of key tile j - 1
         for (int j = 0; j <= nt; ++j) {
+          if (j % kBeatTiles == kBeatTiles - 1 && leader) beat(c->signals);
           if (j > 0 && !full(v)) return;
           if (j < nt && !full(cur)) return;
 #pragma unroll

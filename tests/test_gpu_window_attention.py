@@ -322,6 +322,29 @@ def test_windows_and_sinks_beyond_2_to_the_30(several):
     assert sees(2 * block + 5, window=10, sinks=1 << 40)
 
 
+@pytest.mark.parametrize("n", [3, 200])
+def test_one_item_may_take_longer_than_a_wait(n):
+    """Two heads' queries over 2^28 keys (one page over and over) as one part, because the
+    lengths given are far too small: seconds of key tiles for one CTA, in which the roles
+    that have nothing to do must not give up.  A key at the end outweighs the others."""
+    block, hd, context = 1 << 16, 64, 1 << 28
+    k = torch.zeros((2 * block, 2, hd), dtype=BF16, device="cuda")
+    v = torch.ones_like(k)
+    q = torch.zeros((n, 2, hd), dtype=BF16, device="cuda")
+    q[:, :, 0] = hd ** 0.5
+    k[2 * block - n, :, 0], v[2 * block - n] = 40.0, -2.0     # seen by every query
+    table = torch.zeros((1, context // block), dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    out = torch.full_like(q, float("nan"))
+    window_attention(q, k, v, table, torch.tensor([context], dtype=torch.int32, device="cuda"),
+                     block, max_query_len=1, max_context_len=128, out=out,
+                     cu_seqlens_q=torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    status = ctypes.c_uint32()
+    _lib.check(_lib.lib().ie_kernel_status(ctypes.byref(status), 1))
+    assert status.value == 0
+    assert torch.all(out == -2.0)       # the others weigh 2^28 e^-40 together
+
+
 def test_same_bits_twice_and_on_another_stream():
     b = Batch([700, 3000], 8, 2, 128, BF16, 16, seed=13)
     a = check(b, window=1000, sinks=4)
